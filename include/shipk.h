@@ -45,6 +45,7 @@ extern "C" {
 
 #define SHIPK_DTYPE_F32 0
 #define SHIPK_DTYPE_F16 1
+#define SHIPK_DTYPE_BF16 2 /* a model's scores and results only, not images */
 
 /* One uint8 BGR HWC frame in device memory. */
 typedef struct {
@@ -217,6 +218,76 @@ SHIPK_API int shipk_mask_area(const float* rows, int candidates, int stride, int
                               const float* protos, int channels, int cells, int count,
                               float score_threshold, float mask_threshold, int crop_height,
                               int crop_width, float* areas, void* stream);
+
+/* ---- a model's scores: token log-probabilities ------------------------------------------ */
+
+/* Rows of scores over a vocabulary -> what a reader or captioner answered, on the device. No
+ * counterpart in the reference, whose heads end in host code. logits: device [rows, vocab] of
+ * `dtype` (SHIPK_DTYPE_F32, _F16 or _BF16), rows `row_stride` elements apart. With y = logit /
+ * temperature over the row's allowed tokens and lse = log(sum of e^y):
+ *   logprobs [rows, n_tokens]: y_t - lse of each given token (device int64 [rows, n_tokens]);
+ *     -inf for a token that is not allowed, 0 for a negative token (padding: nothing was given),
+ *     NaN for one past the vocabulary;
+ *   entropy [rows]: lse - (sum of p y), in nats;
+ *   top_ids, top_logprobs [rows, top]: the `top` largest logits among the allowed, equal ones by
+ *     the lower id, with their log-probabilities; id -1 and -inf past the last one.
+ * allowed: device uint32 bit masks, token v is bit v % 32 of word v / 32, rows `allowed_stride`
+ * words apart (0: one mask for every row), or NULL: all. A logit of -inf is not allowed either,
+ * whatever its bit; values at cleared bits, NaN and infinities among them, do not matter. A row
+ * with nothing allowed has log-probabilities -inf, entropy 0 and no alternatives. A NaN or +inf
+ * among the allowed makes the row's log-probabilities and entropy NaN; a NaN is no alternative.
+ * Sums are held in 32 bits relative to the maximum. top <= 64 (else SHIPK_ERANGE) and <= vocab;
+ * temperature in [1e-6, 1e6]. tokens and logprobs may be NULL when n_tokens is 0, top_ids and
+ * top_logprobs when top is 0. Outputs must not overlap inputs. One launch, no workspace. */
+SHIPK_API int shipk_token_logprobs(const void* logits, int dtype, int rows, int vocab, int64_t row_stride,
+                                   const int64_t* tokens, int n_tokens, const uint32_t* allowed,
+                                   int64_t allowed_stride, float temperature, int top, float* logprobs,
+                                   float* entropy, float* top_logprobs, int64_t* top_ids, void* stream);
+
+/* ---- a model's scores: routing rows to experts ------------------------------------------ */
+
+#define SHIPK_SCORES_SOFTMAX 0
+#define SHIPK_SCORES_SIGMOID 1
+#define SHIPK_GROUP_MAX 0  /* a group's score is its best expert's */
+#define SHIPK_GROUP_TOP2 1 /* the sum of its two best (its only one's, where one is left) */
+
+/* A gate's scores -> the experts of each row (a crop's embedders, chosen by score where the
+ * reference's CropStage, stages.cpp:195-245, goes by the class). logits: device [rows, experts]
+ * of `dtype` (F32, F16 or BF16), rows `row_stride` elements apart; bias: device float [experts]
+ * or NULL. Per row, over the experts whose logit and bias are neither -inf nor NaN (+inf counts
+ * as the largest finite logit): score = sigmoid(logit) or softmax over those experts, computed in
+ * 64 bits and rounded once to 32; choice = score + bias, rounded to 32 bits. With groups > 1 the
+ * experts form `groups` runs of equal length and only those of the top_groups best groups
+ * (group_score; ties to the lower group) can be chosen. The top_k largest choices, ties to the
+ * lower expert, go to ids (device int32 [rows, top_k], best first); weights (device float) are
+ * their scores, without the bias, divided by their sum when `renormalise` (0 where that sum is
+ * 0), times `scale`. Past the last expert that can be chosen: id -1, weight 0. Mask an expert
+ * with -inf: a type's lowest finite value is a number, which a bias can still lift.
+ * experts <= 1024, top_k <= 32, groups <= 32 (else SHIPK_ERANGE); top_k <= experts, groups
+ * divides experts, 1 <= top_groups <= groups. Outputs must not overlap inputs. One launch. */
+SHIPK_API int shipk_route_experts(const void* logits, int dtype, int rows, int experts, int64_t row_stride,
+                                  const float* bias, int top_k, int scores, int groups, int top_groups,
+                                  int group_score, int renormalise, float scale, float* weights,
+                                  int32_t* ids, void* stream);
+
+/* Group the rows by expert: a stable sort of the assignments ids (device int32 [rows, k]) by
+ * expert. offsets (device int32 [experts + 1]): expert e's places are [offsets[e], offsets[e+1]).
+ * order (device int32 [rows * k]): the row at each place, ascending within an expert, -1 past
+ * offsets[experts]; what shipk_crop_u8 reads as boxes in this order is each expert's batch.
+ * slots (device int32 [rows, k]): the place of each assignment, -1 where the id is outside
+ * [0, experts) (nothing chosen). experts <= 1024, rows * k <= 2^31 - 2^16 (else SHIPK_ERANGE). Outputs
+ * must not overlap the input. One launch, no workspace, the same result every time. */
+SHIPK_API int shipk_plan_experts(const int32_t* ids, int rows, int k, int experts, int32_t* order,
+                                 int32_t* slots, int32_t* offsets, void* stream);
+
+/* Join the experts' results: out[r] = sum over j of weights[r, j] * in[slots[r, j]], summed in 32
+ * bits in the order of j and rounded once to `dtype` (F32, F16 or BF16). in: device [n_in, width],
+ * rows `row_stride` elements apart, in the plan's order; weights: device float [rows, k]; slots:
+ * device int32 [rows, k], an assignment whose slot is outside [0, n_in) adds nothing, whatever
+ * its weight; out: device [rows, width]. Outputs must not overlap inputs. One launch. */
+SHIPK_API int shipk_combine_experts(const void* in, int dtype, int n_in, int64_t row_stride,
+                                    const float* weights, const int32_t* slots, int rows, int k,
+                                    int width, void* out, void* stream);
 
 /* ---- verification ---------------------------------------------------------------------- */
 

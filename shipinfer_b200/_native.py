@@ -15,6 +15,7 @@ from pathlib import Path
 from shipinfer_b200.errors import ConfigurationError, NativeError, ValidationError
 
 __all__ = [
+    "DTYPE_BF16",
     "DTYPE_F16",
     "DTYPE_F32",
     "FrameNv12",
@@ -30,7 +31,7 @@ _PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("SHIPK_LIBRARY", str(_PKG / "_lib" / "libshipk.so")))
 
 OK, EINVAL, EDEVICE, ECUDA, ERANGE, ENOMEM = 0, 1, 2, 3, 4, 5
-DTYPE_F32, DTYPE_F16 = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
 
 class FrameU8(ctypes.Structure):
@@ -68,6 +69,7 @@ class LetterboxMap(ctypes.Structure):
 _F3 = ctypes.c_float * 3
 _VP = ctypes.c_void_p
 _I = ctypes.c_int
+_I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 _F = ctypes.c_float
 
@@ -114,6 +116,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I,
         [_VP, _I, _I, _I, _VP, _I, _I, _I, _F, _F, _I, _I, _VP, _VP],
     ),
+    "shipk_token_logprobs": (
+        _I,
+        [_VP, _I, _I, _I, _I64, _VP, _I, _VP, _I64, _F, _I, _VP, _VP, _VP, _VP, _VP],
+    ),
+    "shipk_route_experts": (
+        _I,
+        [_VP, _I, _I, _I, _I64, _VP, _I, _I, _I, _I, _I, _I, _F, _VP, _VP, _VP],
+    ),
+    "shipk_plan_experts": (_I, [_VP, _I, _I, _I, _VP, _VP, _VP, _VP]),
+    "shipk_combine_experts": (_I, [_VP, _I, _I, _I64, _VP, _VP, _I, _I, _I, _VP, _VP]),
     "shipk_normalise_check": (_I, [_F, _F, _VP, _VP]),
     "shipk_dp_letterbox_fit": (_I, [_I, _I, _I, _I, ctypes.POINTER(LetterboxMap)]),
     "shipk_dp_letterbox_into": (_I, [_VP, _I, _I, _VP, _I, _I, _I, _F, ctypes.POINTER(LetterboxMap), _VP]),

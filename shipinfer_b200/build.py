@@ -16,8 +16,9 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "libshipk.so"
-SOURCES = ["abi.cu", "letterbox.cu", "crop.cu", "crop_nv12.cu", "nms.cu", "decode.cu", "mask.cu", "selfcheck.cu"]
-HEADERS = ["common.cuh", "kernels.h"]
+SOURCES = ["abi.cu", "letterbox.cu", "crop.cu", "crop_nv12.cu", "nms.cu", "decode.cu", "mask.cu",
+           "logprobs.cu", "routing.cu", "selfcheck.cu"]
+HEADERS = ["common.cuh", "heads.cuh", "kernels.h"]
 PUBLIC_HEADER = PKG.parent / "include" / "shipk.h"
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

@@ -590,6 +590,131 @@ int shipk_mask_area(const float* rows, int candidates, int stride, int prefix, c
     return SHIPK_OK;
 }
 
+// ---- a model's scores ---------------------------------------------------------------------------
+
+namespace {
+
+int element_bytes(int dtype) {
+    return dtype == SHIPK_DTYPE_F32 ? 4 : dtype == SHIPK_DTYPE_F16 || dtype == SHIPK_DTYPE_BF16 ? 2 : 0;
+}
+
+// A device pointer on a boundary of its elements: a kernel's load from any other address faults.
+int check_elements(const void* ptr, int bytes, const char* who, const char* name) {
+    const int rc = check_device_ptr(ptr, who, name);
+    if (rc) return rc;
+    if (reinterpret_cast<uintptr_t>(ptr) % (uintptr_t)bytes)
+        return fail(SHIPK_EINVAL, "%s: %s is not aligned to its %d-byte elements", who, name, bytes);
+    return SHIPK_OK;
+}
+
+}  // namespace
+
+int shipk_token_logprobs(const void* logits, int dtype, int rows, int vocab, int64_t row_stride,
+                         const int64_t* tokens, int n_tokens, const uint32_t* allowed, int64_t allowed_stride,
+                         float temperature, int top, float* logprobs, float* entropy, float* top_logprobs,
+                         int64_t* top_ids, void* stream) {
+    static const char* who = "shipk_token_logprobs";
+    const int size = element_bytes(dtype);
+    if (!size) return fail(SHIPK_EINVAL, "%s: dtype %d is none of F32, F16 and BF16", who, dtype);
+    if (rows < 0 || n_tokens < 0 || top < 0)
+        return fail(SHIPK_EINVAL, "%s: rows %d, tokens %d and top %d must not be negative", who, rows, n_tokens, top);
+    if (vocab < 1) return fail(SHIPK_EINVAL, "%s: a vocabulary of %d tokens is empty", who, vocab);
+    if (vocab > 1 << 30) return fail(SHIPK_ERANGE, "%s: vocabulary %d is above 2^30", who, vocab);
+    if (row_stride < 0 || allowed_stride < 0) return fail(SHIPK_EINVAL, "%s: a stride is negative", who);
+    if (top > vocab) return fail(SHIPK_EINVAL, "%s: top %d is above the vocabulary of %d", who, top, vocab);
+    if (top > kMaxTop) return fail(SHIPK_ERANGE, "%s: top %d is above %d", who, top, kMaxTop);
+    if (!(temperature >= 1e-6f && temperature <= 1e6f))
+        return fail(SHIPK_EINVAL, "%s: temperature %g is outside 1e-6..1e6", who, (double)temperature);
+    if (rows == 0) return SHIPK_OK;
+    int rc;
+    if ((rc = check_elements(logits, size, who, "logits"))) return rc;
+    if ((rc = check_elements(entropy, 4, who, "entropy"))) return rc;
+    if (n_tokens > 0) {
+        if ((rc = check_elements(tokens, 8, who, "tokens"))) return rc;
+        if ((rc = check_elements(logprobs, 4, who, "logprobs"))) return rc;
+    }
+    if (allowed && (rc = check_elements(allowed, 4, who, "allowed"))) return rc;
+    if (top > 0) {
+        if ((rc = check_elements(top_logprobs, 4, who, "top_logprobs"))) return rc;
+        if ((rc = check_elements(top_ids, 8, who, "top_ids"))) return rc;
+    }
+    const Status s = launch_token_logprobs(logits, dtype, rows, vocab, row_stride, tokens, n_tokens, allowed,
+                                           allowed_stride, temperature, top, logprobs, entropy, top_logprobs,
+                                           top_ids, static_cast<cudaStream_t>(stream));
+    return s.code ? fail_status(s, who) : SHIPK_OK;
+}
+
+int shipk_route_experts(const void* logits, int dtype, int rows, int experts, int64_t row_stride, const float* bias,
+                        int top_k, int scores, int groups, int top_groups, int group_score, int renormalise,
+                        float scale, float* weights, int32_t* ids, void* stream) {
+    static const char* who = "shipk_route_experts";
+    const int size = element_bytes(dtype);
+    if (!size) return fail(SHIPK_EINVAL, "%s: dtype %d is none of F32, F16 and BF16", who, dtype);
+    if (rows < 0) return fail(SHIPK_EINVAL, "%s: rows %d is negative", who, rows);
+    if (experts < 1 || top_k < 1 || top_k > experts)
+        return fail(SHIPK_EINVAL, "%s: top_k %d is outside 1..%d experts", who, top_k, experts);
+    if (experts > kMaxExperts) return fail(SHIPK_ERANGE, "%s: %d experts are above %d", who, experts, kMaxExperts);
+    if (top_k > kMaxChosen) return fail(SHIPK_ERANGE, "%s: top_k %d is above %d", who, top_k, kMaxChosen);
+    if (groups < 1 || experts % groups)
+        return fail(SHIPK_EINVAL, "%s: %d groups do not divide %d experts", who, groups, experts);
+    if (groups > kMaxGroups) return fail(SHIPK_ERANGE, "%s: %d groups are above %d", who, groups, kMaxGroups);
+    if (top_groups < 1 || top_groups > groups)
+        return fail(SHIPK_EINVAL, "%s: top_groups %d is outside 1..%d groups", who, top_groups, groups);
+    if (scores != SHIPK_SCORES_SOFTMAX && scores != SHIPK_SCORES_SIGMOID)
+        return fail(SHIPK_EINVAL, "%s: scores %d is neither softmax nor sigmoid", who, scores);
+    if (group_score != SHIPK_GROUP_MAX && group_score != SHIPK_GROUP_TOP2)
+        return fail(SHIPK_EINVAL, "%s: group_score %d is neither max nor top2", who, group_score);
+    if (row_stride < 0) return fail(SHIPK_EINVAL, "%s: row_stride is negative", who);
+    if (rows == 0) return SHIPK_OK;
+    int rc;
+    if ((rc = check_elements(logits, size, who, "logits"))) return rc;
+    if (bias && (rc = check_elements(bias, 4, who, "bias"))) return rc;
+    if ((rc = check_elements(weights, 4, who, "weights"))) return rc;
+    if ((rc = check_elements(ids, 4, who, "ids"))) return rc;
+    const Status s = launch_route(logits, dtype, rows, experts, row_stride, bias, top_k,
+                                  scores == SHIPK_SCORES_SIGMOID, groups, top_groups, group_score == SHIPK_GROUP_TOP2,
+                                  renormalise != 0, scale, weights, ids, static_cast<cudaStream_t>(stream));
+    return s.code ? fail_status(s, who) : SHIPK_OK;
+}
+
+int shipk_plan_experts(const int32_t* ids, int rows, int k, int experts, int32_t* order, int32_t* slots,
+                       int32_t* offsets, void* stream) {
+    static const char* who = "shipk_plan_experts";
+    if (rows < 0 || k < 1) return fail(SHIPK_EINVAL, "%s: rows %d or k %d is out of range", who, rows, k);
+    if (experts < 1) return fail(SHIPK_EINVAL, "%s: %d experts", who, experts);
+    if (experts > kMaxExperts) return fail(SHIPK_ERANGE, "%s: %d experts are above %d", who, experts, kMaxExperts);
+    if ((int64_t)rows * k > 0x7fffffff - 0x10000)
+        return fail(SHIPK_ERANGE, "%s: %d rows of %d assignments are above 2^31 - 2^16", who, rows, k);
+    int rc;
+    if ((rc = check_elements(offsets, 4, who, "offsets"))) return rc;
+    if (rows > 0) {
+        if ((rc = check_elements(ids, 4, who, "ids"))) return rc;
+        if ((rc = check_elements(order, 4, who, "order"))) return rc;
+        if ((rc = check_elements(slots, 4, who, "slots"))) return rc;
+    }
+    const Status s = launch_plan(ids, rows, k, experts, order, slots, offsets, static_cast<cudaStream_t>(stream));
+    return s.code ? fail_status(s, who) : SHIPK_OK;
+}
+
+int shipk_combine_experts(const void* in, int dtype, int n_in, int64_t row_stride, const float* weights,
+                          const int32_t* slots, int rows, int k, int width, void* out, void* stream) {
+    static const char* who = "shipk_combine_experts";
+    const int size = element_bytes(dtype);
+    if (!size) return fail(SHIPK_EINVAL, "%s: dtype %d is none of F32, F16 and BF16", who, dtype);
+    if (rows < 0 || n_in < 0 || k < 1 || width < 0)
+        return fail(SHIPK_EINVAL, "%s: rows %d, results %d, k %d or width %d is out of range", who, rows, n_in, k, width);
+    if (row_stride < 0) return fail(SHIPK_EINVAL, "%s: row_stride is negative", who);
+    if (rows == 0 || width == 0) return SHIPK_OK;
+    int rc;
+    if (n_in > 0 && (rc = check_elements(in, size, who, "in"))) return rc;
+    if ((rc = check_elements(weights, 4, who, "weights"))) return rc;
+    if ((rc = check_elements(slots, 4, who, "slots"))) return rc;
+    if ((rc = check_elements(out, size, who, "out"))) return rc;
+    const Status s = launch_combine(in, dtype, n_in, row_stride, weights, slots, rows, k, width, out,
+                                    static_cast<cudaStream_t>(stream));
+    return s.code ? fail_status(s, who) : SHIPK_OK;
+}
+
 // ---- the C++ data plane's per-frame calls (reference csrc/shipinfer/runtime/ops.h:38-120) ----
 
 namespace {

@@ -89,6 +89,26 @@ Status launch_mask_area(const float* rows, int crops, int candidates, int stride
                         float mask_threshold, int crop_height, int crop_width, float* areas,
                         cudaStream_t stream);
 
+// Scores over a vocabulary -> log-probabilities of given tokens, entropy, top alternatives per row.
+Status launch_token_logprobs(const void* logits, int dtype, int rows, int vocab, int64_t row_stride,
+                             const int64_t* tokens, int n_tokens, const uint32_t* allowed, int64_t allowed_stride,
+                             float temperature, int top, float* logprobs, float* entropy, float* top_logprobs,
+                             int64_t* top_ids, cudaStream_t stream);
+
+constexpr int kMaxTop = 64;        // alternatives of a row
+constexpr int kMaxExperts = 1024;  // experts of a gate
+constexpr int kMaxChosen = 32;     // experts of a row
+constexpr int kMaxGroups = 32;     // groups of experts
+
+// A gate's scores -> each row's experts and weights; the assignments by expert; the results joined.
+Status launch_route(const void* logits, int dtype, int rows, int experts, int64_t row_stride, const float* bias,
+                    int top_k, int sigmoid, int groups, int top_groups, int group_top2, int renormalise, float scale,
+                    float* weights, int32_t* ids, cudaStream_t stream);
+Status launch_plan(const int32_t* ids, int rows, int k, int experts, int32_t* order, int32_t* slots, int32_t* offsets,
+                   cudaStream_t stream);
+Status launch_combine(const void* in, int dtype, int n_in, int64_t row_stride, const float* weights, const int32_t* slots,
+                      int rows, int k, int width, void* out, cudaStream_t stream);
+
 // The allocation-free NMS entry point's scratch: a static device array of
 // nms_static_capacity() bytes, its address on the current device (taken once per device).
 size_t nms_static_capacity();
