@@ -12,8 +12,8 @@
 // when a logit is so far above it that the sums could overflow: a raise rescales them, as a
 // running maximum would at every new one. The threads' sums meet by one rescaling each.
 //
-// The alternatives come out of the same pass. It keeps each thread's largest logit, with its
-// place, and a 16-bit mark for each run of granules that the thread read: the largest logit there. A
+// The alternatives come out of the same pass. It keeps each thread's largest logit, and a 16-bit
+// mark for each run of granules that the thread read: the largest logit there, rounded down. A
 // bound t that at least `top` of the threads' maxima reach is reached by every alternative, and
 // only runs whose mark reaches it can hold one. These few runs are read again (from L2), what
 // reaches t is collected, and the few dozen collected are ranked.
@@ -30,11 +30,12 @@ namespace shipk {
 
 namespace {
 
-constexpr int kThreads = 256;  // per CTA
+constexpr int kWarpCta = 256;  // threads of a CTA whose warps each have a row of their own
 constexpr int kMaxCluster = 8;
-constexpr int kUnroll = 4;     // 16-byte loads of a stage
+constexpr int kUnroll = 4;     // granules (16 bytes) of a thread in a stage
+constexpr int kUnrollLog = 2;
 constexpr int kStages = 2;     // stages a thread has in flight
-static_assert(kUnroll == 4, "a stage is 2^2 granules of a thread");
+static_assert(kUnroll == 1 << kUnrollLog, "");
 
 struct Args {
     const void* logits;
@@ -71,19 +72,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// Two 32-bit values to one instruction: a * b + c, a * b and a + b, each rounded once.
+// Two 32-bit values to one instruction: a * b + c and a + b, each rounded once.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;"
         : "=l"(reinterpret_cast<uint64_t&>(r))
         : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
     return r;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -93,9 +87,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
     return r;
 }
-
-// 2^y below this adds nothing to a sum that holds its reference; the clamp keeps 0 * -inf out.
-constexpr float kLowest = -150.f;
 
 // The parts of LANES neighbouring lanes as one, in each of them: their maximum first, then every
 // part rescaled to it once, then plain sums.
@@ -122,45 +113,137 @@ __device__ __forceinline__ Part join(Part p, float scale) {
     return r;
 }
 
-// The 16 bytes at a granule of the row's memory as float values.
-__device__ __forceinline__ void unpack(const uint4& u, float (&x)[4], const float*) {
-    x[0] = __uint_as_float(u.x);
-    x[1] = __uint_as_float(u.y);
-    x[2] = __uint_as_float(u.z);
-    x[3] = __uint_as_float(u.w);
-}
-__device__ __forceinline__ void unpack(const uint4& u, float (&x)[8], const __half*) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(reinterpret_cast<const __half2&>(w[i]));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-    }
-}
-__device__ __forceinline__ void unpack(const uint4& u, float (&x)[8], const __nv_bfloat16*) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
+// ---- 16 bytes of scores: one granule ----------------------------------------------------------
 
-__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
-                 : "memory");
+template <typename T>
+struct Granule;
+
+// 32-bit scores. `low` stands in for what has no probability: its 2^y is 0 and y 2^y no NaN.
+template <>
+struct Granule<float> {
+    static constexpr int kVec = 4;
+    static __device__ __forceinline__ uint4 empty() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+    static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[4]) {
+        x[0] = __uint_as_float(u.x);
+        x[1] = __uint_as_float(u.y);
+        x[2] = __uint_as_float(u.z);
+        x[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ float largest(const uint4 (&u)[kUnroll]) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+            m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(u[k].x), __uint_as_float(u[k].y)),
+                               fmaxf(__uint_as_float(u[k].z), __uint_as_float(u[k].w))));
+        return m;
+    }
+    // y = x scale + offset of each score, at least -150
+    static __device__ __forceinline__ void scaled(const uint4& u, float2 scale, float2 offset, float2 (&y)[2]) {
+        y[0] = fma2(float2{__uint_as_float(u.x), __uint_as_float(u.y)}, scale, offset);
+        y[1] = fma2(float2{__uint_as_float(u.z), __uint_as_float(u.w)}, scale, offset);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) y[i] = {max_nan(y[i].x, -150.f), max_nan(y[i].y, -150.f)};
+    }
+    // whether scaled() may be used with a reference: x scale does not overflow above, -inf is no trouble
+    static __device__ __forceinline__ bool plain(float, float) { return true; }
+    static __device__ __forceinline__ uint4 cover(const uint4& u, uint32_t bits) {
+        const uint32_t none = 0xff800000u;
+        return make_uint4(bits & 1u ? u.x : none, bits & 2u ? u.y : none, bits & 4u ? u.z : none, bits & 8u ? u.w : none);
+    }
+};
+
+// 16-bit scores, two to a register: the maximum and the clamp at `kLow` are taken on both at once.
+template <typename T>
+struct Granule16 {
+    static constexpr int kVec = 8;
+    static __device__ __forceinline__ uint4 empty() { return make_uint4(T::kNone, T::kNone, T::kNone, T::kNone); }
+    static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = T::both(w[i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ float largest(const uint4 (&u)[kUnroll]) {
+        uint32_t m = T::max2(T::max2(u[0].x, u[0].y), T::max2(u[0].z, u[0].w));
+#pragma unroll
+        for (int k = 1; k < kUnroll; ++k)
+            m = T::max2(m, T::max2(T::max2(u[k].x, u[k].y), T::max2(u[k].z, u[k].w)));
+        const float2 f = T::both(m);
+        return fmaxf(fmaxf(f.x, f.y), -INFINITY);
+    }
+    static __device__ __forceinline__ void scaled(const uint4& u, float2 scale, float2 offset, float2 (&y)[4]) {
+        y[0] = fma2(T::both(T::raise(u.x)), scale, offset);
+        y[1] = fma2(T::both(T::raise(u.y)), scale, offset);
+        y[2] = fma2(T::both(T::raise(u.z)), scale, offset);
+        y[3] = fma2(T::both(T::raise(u.w)), scale, offset);
+    }
+    // with this reference, a score at the clamp or below has no probability
+    static __device__ __forceinline__ bool plain(float ref, float scale) { return (T::kLow - ref) * scale < -150.f; }
+    static __device__ __forceinline__ uint4 cover(const uint4& u, uint32_t bits) {
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t on = (bits >> (2 * i) & 1u ? 0xffffu : 0u) | (bits >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+            w[i] = (w[i] & on) | (T::kNone & ~on);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+struct Bf16Pair {
+    static constexpr uint32_t kNone = 0xff80ff80u;
+    static constexpr float kLow = -1.0101590720568703e30f;  // 0xf14c: any far value whose y stays finite
+    static __device__ __forceinline__ float2 both(uint32_t w) {
+        return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+    }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t raise(uint32_t a) {
+        uint32_t r;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xf14cf14cu));
+        return r;
+    }
+};
+struct HalfPair {
+    static constexpr uint32_t kNone = 0xfc00fc00u;
+    static constexpr float kLow = -65504.f;
+    static __device__ __forceinline__ float2 both(uint32_t w) { return __half22float2(reinterpret_cast<const __half2&>(w)); }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t raise(uint32_t a) {
+        uint32_t r;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xfbfffbffu));
+        return r;
+    }
+};
+template <>
+struct Granule<__nv_bfloat16> : Granule16<Bf16Pair> {};
+template <>
+struct Granule<__half> : Granule16<HalfPair> {};
+
+__device__ __forceinline__ void copy_async(uint32_t to, const uint4* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// ---- a row ------------------------------------------------------------------------------------
 
 // A row's memory in 16-byte granules from the one that holds its first value: granule g holds
 // the values [g kVec - shift, (g + 1) kVec - shift) of the row, those of the first and the last
 // granule that lie outside it excepted.
 template <typename T, bool MASK>
 struct Row {
-    static constexpr int kVec = 16 / sizeof(T);
+    static constexpr int kVec = Granule<T>::kVec;
     const T* x;
     const uint4* base;
     const uint32_t* allowed;
@@ -179,23 +262,17 @@ struct Row {
     }
     __device__ __forceinline__ bool on(int v) const { return !MASK || ((__ldg(allowed + (v >> 5)) >> (v & 31)) & 1u); }
     __device__ __forceinline__ float logit(int v) const { return on(v) ? to_f32(x[v]) : -INFINITY; }
-    __device__ __forceinline__ uint32_t bits(int g) const {  // of a full granule
+    // a full granule's bytes with what is not allowed at -inf
+    __device__ __forceinline__ uint4 cover(const uint4& u, int g) const {
+        if (!MASK) return u;
         const int v = g * kVec - shift, off = v & 31;
         const uint32_t* w = allowed + (v >> 5);
-        return __funnelshift_r(__ldg(w), off + kVec > 32 ? __ldg(w + 1) : 0u, off);
+        return Granule<T>::cover(u, __funnelshift_r(__ldg(w), off + kVec > 32 ? __ldg(w + 1) : 0u, off));
     }
-    __device__ __forceinline__ void cover(int g, float (&v)[kVec]) const {
-        if (MASK) {
-            const uint32_t b = bits(g);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) v[i] = (b >> i) & 1u ? v[i] : -INFINITY;
-        }
-    }
-    // any granule; -inf outside the row
+    // any granule's scores; -inf outside the row
     __device__ __forceinline__ void read(int g, float (&v)[kVec]) const {
         if (g >= full0 && g < full1) {
-            unpack(__ldg(base + g), v, x);
-            cover(g, v);
+            Granule<T>::unpack(cover(__ldg(base + g), g), v);
             return;
         }
 #pragma unroll
@@ -206,6 +283,126 @@ struct Row {
     }
 };
 
+// The granules [g0, g1) of a row that a group works on: the full ones, [from, to), in strides of
+// THREADS, and the row's first and last one, where they are shared with other rows, by the first
+// and the last thread.
+template <typename T, bool MASK, int THREADS>
+struct Run {
+    int g0, g1, from, to;
+
+    __device__ __forceinline__ Run(const Row<T, MASK>& r, unsigned rank, unsigned ranks) {
+        const int each = ranks == 1 ? r.granules : ((r.granules + (int)ranks - 1) / (int)ranks + 7) & ~7;
+        g0 = min(r.granules, each * (int)rank);
+        g1 = min(r.granules, g0 + each);
+        from = max(g0, r.full0);
+        to = min(g1, r.full1);
+    }
+    __device__ __forceinline__ bool first(const Row<T, MASK>& r, int thread) const {
+        return thread == 0 && g0 < min(g1, r.full0);
+    }
+    __device__ __forceinline__ bool last(const Row<T, MASK>& r, int thread) const {
+        return thread == THREADS - 1 && g0 < g1 && r.full1 < g1 && r.full1 >= r.full0;
+    }
+};
+
+// What a thread has of a row while it reads its granules: the sums relative to `ref`, in pairs, and
+// its largest logit. Two ways to add scores. The plain one takes y = x scale + offset in one
+// rounding, with offset = -ref scale rounded: the sums are then relative to the logit whose y is exactly
+// 0, `slip` (in y) away from ref, which part() puts right. The careful one takes (x - ref) scale
+// and clamps each y: for the first scores, where there is no reference yet, for references so
+// large that ref scale says nothing about x scale, and, in 16 bits, for references so low that
+// a score of -inf clamped to a finite one would count.
+template <typename T>
+struct Running {
+    static constexpr int kVec = Granule<T>::kVec;
+    float ref = -INFINITY, best = -INFINITY;
+    float limit = NAN;  // what a logit may reach the plain way; NaN: the careful way
+    float offset = 0.f;
+    float2 s2 = {0.f, 0.f}, h2 = {0.f, 0.f};
+
+    __device__ __forceinline__ void shift(float d) {  // to a reference d lower, in y
+        const float e = exp2_fast(d);
+        h2 = {e * (h2.x + d * s2.x), e * (h2.y + d * s2.y)};
+        s2 = {e * s2.x, e * s2.y};
+    }
+    __device__ __forceinline__ float slip(float scale) const { return -__fmaf_rn(ref, scale, offset); }
+
+    // a reference that suits scores of up to `top`, and whether it serves the plain way
+    __device__ __forceinline__ void raise(float top, float scale, float headroom) {
+        if (limit == limit) {
+            shift(slip(scale));
+            limit = NAN;
+        }
+        if (ref == -INFINITY) {
+            ref = top;
+        } else if (top > ref + headroom) {
+            shift(fmaxf((ref - top) * scale, -1e4f));
+            ref = top;
+        }
+        const float y = ref * scale;
+        if (fabsf(y) < 4194304.f && Granule<T>::plain(ref, scale)) {  // slip below a half
+            offset = -y;
+            shift(-slip(scale));
+            limit = ref + headroom;
+        }
+    }
+    __device__ __forceinline__ void add_carefully(const float (&x)[kVec], float scale) {
+        const float from = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            const float y = max_nan((x[i] - from) * scale, -150.f), e = exp2_fast(y);
+            s2.x += e;
+            h2.x = __fmaf_rn(e, y, h2.x);
+        }
+    }
+    // a stage; returns its largest logit
+    __device__ __forceinline__ float take(const uint4 (&u)[kUnroll], float scale, float headroom) {
+        const float top = Granule<T>::largest(u);
+        best = fmaxf(best, top);
+        if (!(top <= limit)) {
+            raise(top, scale, headroom);
+            if (limit != limit) {
+#pragma unroll 1
+                for (int k = 0; k < kUnroll; ++k) {
+                    const uint4 v = k == 0 ? u[0] : k == 1 ? u[1] : k == 2 ? u[2] : u[3];
+                    float x[kVec];
+                    Granule<T>::unpack(v, x);
+                    add_carefully(x, scale);
+                }
+                return top;
+            }
+        }
+        const float2 scale2 = {scale, scale}, offset2 = {offset, offset};
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            float2 y[kVec / 2];
+            Granule<T>::scaled(u[k], scale2, offset2, y);
+#pragma unroll
+            for (int i = 0; i < kVec / 2; ++i) {
+                const float2 e = {exp2_fast(y[i].x), exp2_fast(y[i].y)};
+                s2 = add2(s2, e);
+                h2 = fma2(e, y[i], h2);
+            }
+        }
+        return top;
+    }
+    __device__ __forceinline__ void take_edge(const float (&x)[kVec], float scale, float headroom) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) top = fmaxf(top, x[i]);
+        best = fmaxf(best, top);
+        // sums relative to ref itself, then the careful way
+        raise(top, scale, headroom);
+        if (limit == limit) shift(slip(scale));
+        add_carefully(x, scale);
+        if (limit == limit) shift(-slip(scale));
+    }
+    __device__ __forceinline__ Part part(float scale) {
+        if (limit == limit) shift(slip(scale));
+        return Part{ref, s2.x + s2.y, h2.x + h2.y};
+    }
+};
+
 // What a group of THREADS threads shares while it works on a row (or a cluster's part of one).
 template <int THREADS>
 struct Shared {
@@ -213,14 +410,13 @@ struct Shared {
     static constexpr int kMarks = THREADS == 32 ? 8 : 16;  // of a thread
     uint64_t keys[kCollect];           // the logits that reach the bound
     uint64_t chosen[kMaxTop];
-    uint64_t rounds[THREADS / 32];     // a warp's contribution to the bound
     Part parts[THREADS / 32];
+    uint32_t rounds[THREADS / 32];     // a warp's contribution to the bound
     uint32_t ord[THREADS];             // order bits of the threads' maxima, 0: none
-    int at[THREADS];                   // and their granules
     uint16_t marks[kMarks * THREADS];  // upper half of the order bits of a run's largest logit
     uint16_t runs[kCollect];           // marked runs to read again: mark * THREADS + thread
     int marked, collected;
-    uint64_t bound;
+    uint32_t bound;
 };
 
 template <int THREADS>
@@ -229,17 +425,11 @@ __device__ __forceinline__ void group_sync() {
     else __syncthreads();
 }
 
-// A bound is a key: order bits of a logit, then its granule, the lower the better. What reaches it
-// is a larger logit, or the same one in that granule or before; 0 is reached by every logit.
-__device__ __forceinline__ uint64_t bound_key(uint32_t ord, int at) {
-    return ord ? ((uint64_t)ord << 32) | (0xffffffffu - (uint32_t)at) : 0;
-}
-
-// A bound that at least `wanted` of the threads' maxima reach, and few more: the search ends as soon
-// as their number is within an eighth. Run by one warp, on g.ord and g.at. 0 when fewer than `wanted` threads
-// have any logit.
+// Order bits that at least `wanted` of the threads' maxima reach, and few more where they differ: the
+// search ends as soon as their number is within an eighth. Run by one warp, on g.ord. 0 when
+// fewer than `wanted` threads have any logit.
 template <int THREADS>
-__device__ __forceinline__ uint64_t find_bound(const Shared<THREADS>& g, int wanted, int lane) {
+__device__ __forceinline__ uint32_t find_bound(const Shared<THREADS>& g, int wanted, int lane) {
     constexpr int N = THREADS / 32;
     auto sum = [](int n) {
         if constexpr (N == 1) return __popc(__ballot_sync(0xffffffffu, n));
@@ -277,160 +467,159 @@ __device__ __forceinline__ uint64_t find_bound(const Shared<THREADS>& g, int wan
             reach = n;
         }
     }
-    int last = 0x7fffffff;
-    if (reach > enough) {  // many equal ones: those in the first granules
-        int above = 0, lo = 0x7fffffff, hi = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            above += o[i] > t;
-            if (o[i] == t) {
-                lo = min(lo, g.at[lane + 32 * i]);
-                hi = max(hi, g.at[lane + 32 * i]);
-            }
-        }
-        above = sum(above);
-        lo = __reduce_min_sync(0xffffffffu, lo) - 1;
-        last = __reduce_max_sync(0xffffffffu, hi);
-        while (last - lo > 1 && reach > enough) {  // those up to `last` suffice, those up to `lo` do not
-            const int mid = lo + (last - lo) / 2;
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < N; ++i) n += o[i] == t && g.at[lane + 32 * i] <= mid;
-            n = above + sum(n);
-            if (n >= wanted) {
-                last = mid;
-                reach = n;
-            } else {
-                lo = mid;
-            }
-        }
-    }
-    return bound_key(t, last);
+    return t;
 }
 
-// The same for a group of several warps without a search: with q = wanted / warps rounded up, the least
-// of the warps' q-th largest maxima. Looser (some two times `wanted` reach it), far shorter. 0 when a
-// warp has fewer than q. The warp's part: its q-th largest.
-__device__ __forceinline__ uint64_t nth_largest(uint32_t ord, int at, int q, int lane) {
+// A group of several warps has a bound without that search: with q = wanted / warps rounded up, the
+// least of the warps' q-th largest maxima. Looser (some two times `wanted` reach it), far
+// shorter. 0 when a warp has fewer than q logits. This is a warp's part of it.
+__device__ __forceinline__ uint32_t nth_largest(uint32_t ord, int q, int lane) {
     uint32_t high = 0;
-    int low = 0;
     for (int i = 0; i < q; ++i) {
         high = __reduce_max_sync(0xffffffffu, ord);
-        low = __reduce_min_sync(0xffffffffu, ord == high ? at : 0x7fffffff);
-        if (ord == high && at == low) ord = 0;
+        if (lane == __ffs(__ballot_sync(0xffffffffu, ord == high)) - 1) ord = 0;
     }
-    return bound_key(high, low);
+    return high;
 }
 
-template <int VEC>
-__device__ __forceinline__ float largest(const float (&x)[VEC]) {
-    const float m = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    if constexpr (VEC == 8) return fmaxf(m, fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    return m;
-}
-
-// What a thread has of a row's sums and its largest logit while it reads its granules.
-template <int VEC>
-struct Running {
-    float ref = -INFINITY, limit = -INFINITY, best = -INFINITY;
-    int best_at = 0;
-    float2 s2 = {0.f, 0.f}, h2 = {0.f, 0.f}, minus_ref = {0.f, 0.f};
-
-    __device__ __forceinline__ float take(const float (&x)[VEC], int at, float scale, float headroom) {
-        const float top = largest(x);
-        if (top > best) {
-            best = top;
-            best_at = at;
-        }
-        if (top > limit) {  // the first logit, or one far above the reference
-            const float d = fmaxf((ref - top) * scale, -1e4f);
-            if (ref > -INFINITY) {
-                const float e = exp2_fast(d);
-                h2 = {e * (h2.x + d * s2.x), e * (h2.y + d * s2.y)};
-                s2 = {e * s2.x, e * s2.y};
-            }
-            ref = top;
-            limit = top + headroom;
-            minus_ref = {-top, -top};
-        }
-        const float2 scale2 = {scale, scale};
+template <int THREADS>
+__device__ __forceinline__ uint64_t group_max(Shared<THREADS>& g, uint64_t k, int tid) {
 #pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-            // the difference first: a product with the scale may round away what is left of it
-            float2 y = mul2(add2(float2{x[i], x[i + 1]}, minus_ref), scale2);
-            y = {max_nan(y.x, kLowest), max_nan(y.y, kLowest)};
-            const float2 e = {exp2_fast(y.x), exp2_fast(y.y)};
-            s2 = add2(s2, e);
-            h2 = fma2(e, y, h2);
-        }
-        return top;
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t c = __shfl_xor_sync(0xffffffffu, k, o);
+        k = c > k ? c : k;
     }
-    __device__ __forceinline__ Part part() const { return Part{ref, s2.x + s2.y, h2.x + h2.y}; }
-};
+    if (THREADS == 32) return k;
+    __syncthreads();
+    if ((tid & 31) == 0) g.keys[tid / 32] = k;
+    __syncthreads();
+    for (int w = 0; w < THREADS / 32; ++w) k = g.keys[w] > k ? g.keys[w] : k;
+    return k;
+}
 
-// The granules [g0, g1) of a row that a group works on: the full ones in strides of THREADS, and
-// the row's first and last one, where they are shared with other rows, by the first and the last
-// thread.
+// The alternatives one after another, the best below the one before each time: for rows where more
+// reaches the bound than the group can hold (large logits gathered in few threads' places).
 template <typename T, bool MASK, int THREADS>
-struct Run {
-    int g0, g1, from, to;
+__device__ __noinline__ void choose_slowly(Shared<THREADS>& g, Row<T, MASK> r, Run<T, MASK, THREADS> run,
+                                           int wanted, int tid) {
+    constexpr int kVec = Row<T, MASK>::kVec;
+    uint64_t before = ~0ull;
+    for (int j = 0; j < wanted && before; ++j) {
+        uint64_t k = 0;
+        for (int at = run.g0 + tid; at < run.g1; at += THREADS) {
+            float x[kVec];
+            r.read(at, x);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                if (!(x[i] > -INFINITY)) continue;
+                const uint64_t c = choice_key(x[i], at * kVec - r.shift + i);
+                if (c < before && c > k) k = c;
+            }
+        }
+        k = group_max<THREADS>(g, k, tid);
+        if (tid == 0) g.chosen[j] = k;
+        before = k;
+    }
+}
 
-    __device__ __forceinline__ Run(const Row<T, MASK>& r, unsigned rank, unsigned ranks) {
-        const int each = ranks == 1 ? r.granules : ((r.granules + (int)ranks - 1) / (int)ranks + 7) & ~7;
-        g0 = min(r.granules, each * (int)rank);
-        g1 = min(r.granules, g0 + each);
-        from = max(g0, r.full0);
-        to = min(g1, r.full1);
+// For rows where many logits equal the bound t (rows of one value, zeros): what is above t as ever,
+// and the first that equal it, found in the row's order until there are enough. False if more is above
+// t than the group can hold.
+template <typename T, bool MASK, int THREADS>
+__device__ __noinline__ bool collect_ties(Shared<THREADS>& g, Row<T, MASK> r, Run<T, MASK, THREADS> run,
+                                          int wanted, int tid, uint32_t t) {
+    constexpr int kVec = Row<T, MASK>::kVec;
+    constexpr int kHold = Shared<THREADS>::kCollect;
+    group_sync<THREADS>();
+    if (tid == 0) g.collected = 0;
+    group_sync<THREADS>();
+    for (int at = run.g0 + tid; at < run.g1; at += THREADS) {
+        float x[kVec];
+        r.read(at, x);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            if (!(x[i] > -INFINITY && order_bits(x[i]) > t)) continue;
+            const int n = atomicAdd(&g.collected, 1);
+            if (n < kHold) g.keys[n] = choice_key(x[i], at * kVec - r.shift + i);
+        }
     }
-    __device__ __forceinline__ bool first(const Row<T, MASK>& r, int thread) const {
-        return thread == 0 && g0 < min(g1, r.full0);
+    group_sync<THREADS>();
+    if (g.collected > kHold - kMaxTop) return false;
+    // THREADS granules at a time, in order; each thread's equals are numbered before they are kept
+    int missing = wanted - g.collected;
+    for (int at0 = run.g0; at0 < run.g1 && missing > 0; at0 += THREADS) {
+        float x[kVec];
+        int mine = 0;
+        const int at = at0 + tid;
+        if (at < run.g1) {
+            r.read(at, x);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) mine += x[i] > -INFINITY && order_bits(x[i]) == t;
+        }
+        group_sync<THREADS>();
+        g.ord[tid] = (uint32_t)mine;
+        group_sync<THREADS>();
+        int before = 0, total = 0;
+        for (int i = 0; i < THREADS; ++i) {
+            const int n = (int)g.ord[i];
+            before += i < tid ? n : 0;
+            total += n;
+        }
+        if (mine) {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                if (!(x[i] > -INFINITY && order_bits(x[i]) == t)) continue;
+                if (before < missing) {
+                    const int n = atomicAdd(&g.collected, 1);
+                    g.keys[n] = choice_key(x[i], at * kVec - r.shift + i);
+                }
+                ++before;
+            }
+        }
+        missing -= total;
     }
-    __device__ __forceinline__ bool last(const Row<T, MASK>& r, int thread) const {
-        return thread == THREADS - 1 && g0 < g1 && r.full1 < g1 && r.full1 >= r.full0;
-    }
-};
+    group_sync<THREADS>();
+    return true;
+}
 
 // The alternatives among a run's granules into g.chosen, best first, 0 past the last; called by the
-// whole group with each thread's largest logit and its granule, which are in g.ord and g.at, and, for
-// more than one warp, with the warps' parts of the bound in g.rounds. `marks` runs of 2^shift granules of each thread have marks.
+// whole group with each thread's largest logit, which is in g.ord, and, for more than one warp,
+// with the warps' parts of the bound in g.rounds. Each of a thread's `marks` marks stands for
+// 2^shift granules.
 template <typename T, bool MASK, int THREADS>
 __device__ __forceinline__ void choose(Shared<THREADS>& g, const Row<T, MASK>& r, const Run<T, MASK, THREADS>& run,
-                                       int wanted, int tid, uint32_t ord, int best_at, int marks, int shift) {
+                                       int wanted, int tid, uint32_t ord, int marks, int shift) {
     constexpr int kVec = Row<T, MASK>::kVec;
     constexpr int kWarps = THREADS / 32;
-    const int lane = tid & 31, warp = tid / 32;
-    uint64_t bound;
+    constexpr int kHold = Shared<THREADS>::kCollect;
+    uint32_t t;
     if (kWarps == 1) {
-        bound = find_bound<THREADS>(g, wanted, lane);
+        t = find_bound<THREADS>(g, wanted, tid);
     } else {
-        bound = g.rounds[0];
-        for (int w = 1; w < kWarps; ++w) bound = min(bound, g.rounds[w]);
-        if (!bound) {  // warps with few logits, or none: uniform over the group
-            if (warp == 0) {
-                bound = find_bound<THREADS>(g, wanted, lane);
-                if (lane == 0) g.bound = bound;
+        t = g.rounds[0];
+        for (int w = 1; w < kWarps; ++w) t = min(t, g.rounds[w]);
+        if (!t) {  // warps with few logits, or none: uniform over the group
+            if (tid < 32) {
+                t = find_bound<THREADS>(g, wanted, tid);
+                if (tid == 0) g.bound = t;
             }
-            group_sync<THREADS>();
-            bound = g.bound;
+            __syncthreads();
+            t = g.bound;
         }
     }
-    const uint32_t t = (uint32_t)(bound >> 32);
-    const int last = key_index(bound);
     auto look = [&](const float (&x)[kVec], int at) {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-            if (!(x[i] > -INFINITY)) continue;
-            const uint32_t o = order_bits(x[i]);
-            if (o < t || (o == t && at > last)) continue;
+            if (!(x[i] > -INFINITY && order_bits(x[i]) >= t)) continue;
             const int n = atomicAdd(&g.collected, 1);
-            if (n < Shared<THREADS>::kCollect) g.keys[n] = choice_key(x[i], at * kVec - r.shift + i);
+            if (n < kHold) g.keys[n] = choice_key(x[i], at * kVec - r.shift + i);
         }
     };
-    if (ord && bound_key(ord, best_at) >= bound) {
+    if (ord && ord >= t) {
         for (int m = 0; m < marks; ++m) {
             if (g.marks[m * THREADS + tid] < t >> 16) continue;
             const int n = atomicAdd(&g.marked, 1);
-            if (n < Shared<THREADS>::kCollect) g.runs[n] = (uint16_t)(m * THREADS + tid);
+            if (n < kHold) g.runs[n] = (uint16_t)(m * THREADS + tid);
         }
         if (run.first(r, tid) || run.last(r, tid)) {
             float x[kVec];
@@ -440,19 +629,20 @@ __device__ __forceinline__ void choose(Shared<THREADS>& g, const Row<T, MASK>& r
         }
     }
     group_sync<THREADS>();
-    const int looks = min(g.marked, Shared<THREADS>::kCollect) << shift;
+    const int looks = min(g.marked, kHold) << shift;
     for (int q = tid; q < looks; q += THREADS) {
         const int of = g.runs[q >> shift], k = q & ((1 << shift) - 1);
         const int at = run.from + of % THREADS + (((of / THREADS) << shift) + k) * THREADS;
         if (at >= run.to) continue;
         float x[kVec];
-        unpack(__ldg(r.base + at), x, r.x);
-        r.cover(at, x);
+        Granule<T>::unpack(r.cover(__ldg(r.base + at), at), x);
         look(x, at);
     }
     group_sync<THREADS>();
-    const int n = g.collected;
-    if (n <= Shared<THREADS>::kCollect && g.marked <= Shared<THREADS>::kCollect) {
+    bool held = g.collected <= kHold && g.marked <= kHold;
+    if (!held) held = collect_ties<T, MASK, THREADS>(g, r, run, wanted, tid, t);
+    if (held) {
+        const int n = g.collected;
         for (int i = tid; i < n; i += THREADS) {
             const uint64_t k = g.keys[i];
             int better = 0;
@@ -460,33 +650,7 @@ __device__ __forceinline__ void choose(Shared<THREADS>& g, const Row<T, MASK>& r
             if (better < wanted) g.chosen[better] = k;
         }
     } else {
-        // more than the group can hold reach the bound (large logits gathered in few threads'
-        // places): the best below the one before, again and again
-        uint64_t before = ~0ull;
-        for (int j = 0; j < wanted && before; ++j) {
-            uint64_t k = 0;
-            for (int at = run.g0 + tid; at < run.g1; at += THREADS) {
-                float x[kVec];
-                r.read(at, x);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    if (!(x[i] > -INFINITY)) continue;
-                    const uint64_t c = choice_key(x[i], at * kVec - r.shift + i);
-                    if (c < before && c > k) k = c;
-                }
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const uint64_t c = __shfl_xor_sync(0xffffffffu, k, o);
-                k = c > k ? c : k;
-            }
-            group_sync<THREADS>();
-            if (lane == 0) g.keys[warp] = k;
-            group_sync<THREADS>();
-            for (int w = 0; w < kWarps; ++w) k = g.keys[w] > k ? g.keys[w] : k;
-            if (tid == 0) g.chosen[j] = k;
-            before = k;
-        }
+        choose_slowly<T, MASK, THREADS>(g, r, run, wanted, tid);
     }
     group_sync<THREADS>();
 }
@@ -518,17 +682,22 @@ __device__ __forceinline__ void write_row(const Args& a, const Row<T, MASK>& r, 
 // memory, kStages stages of kUnroll ahead of where it reads, past the end of a row into the next
 // one: what a row needs beyond its pass runs while the next row arrives. No thread reads what
 // another copied, so the copies need no barrier.
+template <int THREADS>
+constexpr int kCta = THREADS == 32 ? kWarpCta : THREADS;
+
 template <typename T, int THREADS, bool MASK, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_kernel(const __grid_constant__ Args a) {
     constexpr int kVec = Row<T, MASK>::kVec;
-    constexpr int kWarps = THREADS / 32, kGroups = kThreads / THREADS;
-    extern __shared__ uint4 rings[];  // [kGroups][kStages][kUnroll][THREADS]
+    constexpr int kWarps = THREADS / 32, kGroups = kCta<THREADS> / THREADS;
+    constexpr int kStage = kUnroll * THREADS;  // granules
+    extern __shared__ uint4 rings[];           // [kGroups][kStages][kUnroll][THREADS]
     __shared__ Shared<THREADS> shared[kGroups];
     __shared__ uint64_t cluster_keys[CLUSTER ? kMaxCluster * kMaxTop : 1];
     __shared__ Part cluster_parts[CLUSTER ? kMaxCluster : 1];
     const int group = threadIdx.x / THREADS, tid = threadIdx.x % THREADS, lane = tid & 31;
     Shared<THREADS>& g = shared[group];
-    uint4* const ring = rings + group * kStages * kUnroll * THREADS + tid;
+    const uint4* const ring = rings + group * kStages * kStage + tid;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     unsigned part = 0, parts = 1;
     if (CLUSTER) {
         cg::cluster_group cluster = cg::this_cluster();
@@ -539,30 +708,33 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const __grid_cons
     const int64_t first = CLUSTER ? blockIdx.x / parts : (int64_t)blockIdx.x * kGroups + group;
     const int64_t step = CLUSTER ? gridDim.x / parts : (int64_t)gridDim.x * kGroups;
 
-    // the next stage to copy: of row `ahead`, granules from `next` to `end`
+    // the next stage to copy: of row `ahead`, its `left` granules from `next` on
     int64_t ahead = first;
-    const uint4* ahead_base = nullptr;
-    int next = 0, end = 0;
+    const uint4* next = nullptr;
+    int left = 0;
     auto enter = [&]() {
         const Row<T, MASK> r(a, ahead);
         const Run<T, MASK, THREADS> run(r, part, parts);
-        ahead_base = r.base + tid;
-        next = run.from;
-        end = run.to;
+        next = r.base + run.from + tid;
+        left = run.to - run.from;
     };
     if (ahead < a.rows) enter();
     auto copy_stage = [&](int stage) {
-        while (ahead < a.rows && next >= end) {
+        while (left <= 0 && ahead < a.rows) {
             ahead += step;
             if (ahead < a.rows) enter();
         }
-        if (ahead < a.rows) {
+        const uint32_t to = ring_at + (uint32_t)(stage * kStage * sizeof(uint4));
+        if (left >= kStage) {
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) copy_async(to + k * THREADS * sizeof(uint4), next + k * THREADS);
+        } else {
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k)
-                if (next + k * THREADS + tid < end)
-                    copy_async(ring + (stage * kUnroll + k) * THREADS, ahead_base + next + k * THREADS);
-            next += kUnroll * THREADS;
+                if (k * THREADS + tid < left) copy_async(to + k * THREADS * sizeof(uint4), next + k * THREADS);
         }
+        next += kStage;
+        left -= kStage;
         copies_commit();
     };
 #pragma unroll
@@ -572,34 +744,30 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const __grid_cons
     for (int64_t row = first; row < a.rows; row += step) {
         const Row<T, MASK> r(a, row);
         const Run<T, MASK, THREADS> run(r, part, parts);
-        Running<kVec> sums;
-        float x[kVec];
+        Running<T> sums;
         if (run.first(r, tid)) {
+            float x[kVec];
             r.read(0, x);
-            sums.take(x, 0, a.scale, a.headroom);
+            sums.take_edge(x, a.scale, a.headroom);
         }
         // marks of 2^per stages each
-        const int stages = (max(0, run.to - run.from) + kUnroll * THREADS - 1) / (kUnroll * THREADS);
+        const int stages = (max(0, run.to - run.from) + kStage - 1) / kStage;
         const int per = stages > Shared<THREADS>::kMarks ? 32 - __clz((stages - 1) / Shared<THREADS>::kMarks) : 0;
         float marked = -INFINITY;
         for (int k0 = 0; k0 < stages; ++k0) {
             copies_wait<kStages - 1>();
-            const uint4* held = ring + stage * kUnroll * THREADS;
-            const int at = run.from + k0 * kUnroll * THREADS + tid;
-            if (at - tid + kUnroll * THREADS <= run.to) {
+            const uint4* held = ring + stage * kStage;
+            const int at = run.from + k0 * kStage + tid;
+            uint4 u[kUnroll];
+            if (at - tid + kStage <= run.to) {
 #pragma unroll
-                for (int k = 0; k < kUnroll; ++k) {
-                    unpack(held[k * THREADS], x, r.x);
-                    r.cover(at + k * THREADS, x);
-                    marked = fmaxf(marked, sums.take(x, at + k * THREADS, a.scale, a.headroom));
-                }
+                for (int k = 0; k < kUnroll; ++k) u[k] = r.cover(held[k * THREADS], at + k * THREADS);
             } else {
-                for (int k = 0; k < kUnroll && at + k * THREADS < run.to; ++k) {
-                    unpack(held[k * THREADS], x, r.x);
-                    r.cover(at + k * THREADS, x);
-                    marked = fmaxf(marked, sums.take(x, at + k * THREADS, a.scale, a.headroom));
-                }
+#pragma unroll
+                for (int k = 0; k < kUnroll; ++k)
+                    u[k] = at + k * THREADS < run.to ? r.cover(held[k * THREADS], at + k * THREADS) : Granule<T>::empty();
             }
+            marked = fmaxf(marked, sums.take(u, a.scale, a.headroom));
             copy_stage(stage);
             stage = stage + 1 == kStages ? 0 : stage + 1;
             if (((k0 + 1) & ((1 << per) - 1)) == 0 || k0 + 1 == stages) {
@@ -608,27 +776,26 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const __grid_cons
             }
         }
         if (run.last(r, tid)) {
+            float x[kVec];
             r.read(run.g1 - 1, x);
-            sums.take(x, run.g1 - 1, a.scale, a.headroom);
+            sums.take_edge(x, a.scale, a.headroom);
         }
-        Part p = join<32>(sums.part(), a.scale);
+        Part p = join<32>(sums.part(a.scale), a.scale);
         const uint32_t ord = sums.best > -INFINITY ? order_bits(sums.best) : 0u;
         if (kWarps > 1 && lane == 0) g.parts[tid / 32] = p;
         if (a.top > 0) {
             g.ord[tid] = ord;
-            g.at[tid] = sums.best_at;
             if (tid == 0) g.marked = g.collected = 0;
             for (int j = tid; j < a.top; j += THREADS) g.chosen[j] = 0;
             if (kWarps > 1) {
-                const uint64_t nth = nth_largest(ord, sums.best_at, (a.top + kWarps - 1) / kWarps, lane);
+                const uint32_t nth = nth_largest(ord, (a.top + kWarps - 1) / kWarps, lane);
                 if (lane == 0) g.rounds[tid / 32] = nth;
             }
         }
         group_sync<THREADS>();
         if (kWarps > 1) p = join<kWarps>(g.parts[lane % kWarps], a.scale);
         if (a.top > 0)
-            choose<T, MASK, THREADS>(g, r, run, a.top, tid, ord, sums.best_at, (stages + (1 << per) - 1) >> per,
-                                     per + 2);
+            choose<T, MASK, THREADS>(g, r, run, a.top, tid, ord, (stages + (1 << per) - 1) >> per, per + kUnrollLog);
         if (CLUSTER) {  // its parts meet in its first CTA
             cg::cluster_group cluster = cg::this_cluster();
             cluster.barrier_wait();
@@ -657,36 +824,20 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const __grid_cons
 }
 
 constexpr int kSms = 148;
-constexpr int kCtas = 4;          // per SM, by the launch bounds and the rings
 constexpr int kWarpVocab = 4096;  // a warp takes rows of up to this many scores
 constexpr int kWarpTop = 20;      // and this many alternatives of its 32 threads' maxima
 
-template <typename T, bool MASK>
-cudaError_t launch(const Args& a, cudaStream_t stream) {
+template <typename T, int THREADS, bool MASK, bool CLUSTER>
+cudaError_t launch(const Args& a, int cluster, cudaStream_t stream) {
+    constexpr int kThreads = kCta<THREADS>, kRows = kThreads / THREADS;
     constexpr int ring = kStages * kUnroll * kThreads * (int)sizeof(uint4);
-    if (a.vocab <= kWarpVocab && a.top <= kWarpTop) {
-        constexpr int rows = kThreads / 32;
-        auto kernel = logprobs_kernel<T, 32, MASK, false>;
-        const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), ring);
-        if (e != cudaSuccess) return e;
-        const int64_t ctas = std::min<int64_t>(((int64_t)a.rows + rows - 1) / rows, kSms * kCtas);
-        kernel<<<(unsigned)ctas, kThreads, ring, stream>>>(a);
-        return cudaGetLastError();
-    }
-    int cluster = 1;
-    while (cluster < kMaxCluster && (int64_t)a.rows * cluster < kSms * 8 && a.vocab / cluster > 4096) cluster *= 2;
-    if (cluster == 1) {
-        auto kernel = logprobs_kernel<T, kThreads, MASK, false>;
-        const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), ring);
-        if (e != cudaSuccess) return e;
-        kernel<<<std::min(a.rows, kSms * kCtas), kThreads, ring, stream>>>(a);
-        return cudaGetLastError();
-    }
-    auto kernel = logprobs_kernel<T, kThreads, MASK, true>;
+    auto kernel = logprobs_kernel<T, THREADS, MASK, CLUSTER>;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), ring);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned)(a.rows * cluster));
+    // as many CTAs as run at once, which walk over the rows; with clusters, all of them
+    config.gridDim = CLUSTER ? dim3((unsigned)(a.rows * cluster))
+                             : dim3((unsigned)std::min<int64_t>(((int64_t)a.rows + kRows - 1) / kRows, kSms * (1024 / kThreads)));
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = ring;
     config.stream = stream;
@@ -694,10 +845,19 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim = {(unsigned)cluster, 1, 1};
     config.attrs = &attr;
-    config.numAttrs = 1;
+    config.numAttrs = CLUSTER ? 1 : 0;
     e = cudaLaunchKernelEx(&config, kernel, a);
     const cudaError_t last = cudaGetLastError();
     return e != cudaSuccess ? e : last;
+}
+
+template <typename T, bool MASK>
+cudaError_t launch(const Args& a, cudaStream_t stream) {
+    if (a.vocab <= kWarpVocab && a.top <= kWarpTop) return launch<T, 32, MASK, false>(a, 1, stream);
+    int cluster = 1;
+    while (cluster < kMaxCluster && (int64_t)a.rows * cluster < kSms * 8 && a.vocab / cluster > 4096) cluster *= 2;
+    if (cluster == 1) return launch<T, 256, MASK, false>(a, 1, stream);
+    return launch<T, 256, MASK, true>(a, cluster, stream);
 }
 
 template <typename T>
