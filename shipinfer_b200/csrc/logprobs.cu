@@ -364,7 +364,9 @@ struct Running {
             if (limit != limit) {
 #pragma unroll 1
                 for (int k = 0; k < kUnroll; ++k) {
-                    const uint4 v = k == 0 ? u[0] : k == 1 ? u[1] : k == 2 ? u[2] : u[3];
+                    uint4 v = u[0];
+#pragma unroll
+                    for (int i = 1; i < kUnroll; ++i) v = i == k ? u[i] : v;
                     float x[kVec];
                     Granule<T>::unpack(v, x);
                     add_carefully(x, scale);
@@ -855,7 +857,7 @@ template <typename T, bool MASK>
 cudaError_t launch(const Args& a, cudaStream_t stream) {
     if (a.vocab <= kWarpVocab && a.top <= kWarpTop) return launch<T, 32, MASK, false>(a, 1, stream);
     int cluster = 1;
-    while (cluster < kMaxCluster && (int64_t)a.rows * cluster < kSms * 8 && a.vocab / cluster > 4096) cluster *= 2;
+    while (cluster < kMaxCluster && (int64_t)a.rows * cluster <= kSms && a.vocab / cluster > 8192) cluster *= 2;
     if (cluster == 1) return launch<T, 256, MASK, false>(a, 1, stream);
     return launch<T, 256, MASK, true>(a, cluster, stream);
 }

@@ -16,6 +16,12 @@
 #include "heads.cuh"
 #include "kernels.h"
 
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+namespace cg = cooperative_groups;
+
 namespace shipk {
 
 namespace {
@@ -30,112 +36,262 @@ struct RouteArgs {
     int rows, experts;
     int64_t row_stride;
     const float* bias;
-    int top_k, sigmoid, groups, top_groups, group_top2, renormalise;
+    int top_k, groups, top_groups, group_top2, renormalise;
+    int each;  // experts of a lane
+    int wide;  // 16 bytes of a lane's logits at a time
     float scale;
     float* weights;
     int32_t* ids;
 };
 
-__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
+__device__ __forceinline__ double exact_logit(float x) { return (double)fminf(x, 3.402823466e38f); }  // +inf: the largest
+__device__ __forceinline__ float exact_sigmoid(float x) { return (float)(1.0 / (1.0 + exp(-exact_logit(x)))); }
+
+// What a warp holds of a row: expert lane * each + i in slot i of a lane. Slots past the experts and
+// experts that cannot be chosen hold a choice of -inf.
+template <int NS>
+struct Choices {
+    float c[NS];
+    uint32_t ord;  // the lane's best: its order bits (0: none) and its slot
+    int slot;
+
+    __device__ __forceinline__ void best() {
+        float m = c[0];
+        slot = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t c = __shfl_xor_sync(0xffffffffu, k, o);
-        k = c > k ? c : k;
+        for (int i = 1; i < NS; ++i)
+            if (c[i] > m) {
+                m = c[i];
+                slot = i;
+            }
+        ord = m > -INFINITY ? order_bits(m) : 0u;
     }
-    return k;
+    __device__ __forceinline__ void drop(int s) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (i == s) c[i] = -INFINITY;
+    }
+};
+
+// The larger two of two descending pairs.
+__device__ __forceinline__ void merge2(float& first, float& second, float f, float s) {
+    second = fmaxf(fminf(first, f), fmaxf(second, s));
+    first = fmaxf(first, f);
 }
 
-// One warp per row; the scores and choices of its row stand in shared memory.
-template <typename T>
+// Closes every group but the top_groups best. With groups of whole lanes a group's score meets in
+// its lanes; else through `row` (shared memory, one float for each expert). Returns how far the last
+// group kept is above the next one.
+template <int NS>
+__device__ __forceinline__ float keep_groups(const RouteArgs& a, Choices<NS>& k, float* row, int lane) {
+    const int size = a.experts / a.groups;
+    float first = -INFINITY, second = -INFINITY;
+    const bool whole = size % a.each == 0;
+    const int span = whole ? size / a.each : 1;  // lanes of a group
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) merge2(first, second, k.c[i], -INFINITY);
+        if ((span & (span - 1)) == 0) {
+            for (int o = 1; o < span; o *= 2)
+                merge2(first, second, __shfl_xor_sync(0xffffffffu, first, o), __shfl_xor_sync(0xffffffffu, second, o));
+        } else {  // a group's first lane gathers the others'
+            const float f = first, s = second;
+            for (int o = 1; o < span; ++o)
+                merge2(first, second, __shfl_down_sync(0xffffffffu, f, o), __shfl_down_sync(0xffffffffu, s, o));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (i < a.each && lane * a.each + i < a.experts) row[lane * a.each + i] = k.c[i];
+        __syncwarp();
+        if (lane < a.groups)
+            for (int i = 0; i < size; ++i) merge2(first, second, row[lane * size + i], -INFINITY);
+    }
+    // lane g takes group g's score as a key; 0: nothing in it can be chosen
+    float value = a.group_top2 && second > -INFINITY ? __fadd_rn(first, second) : first;
+    uint64_t key = first > -INFINITY ? 1 : 0;
+    const int from = whole ? lane * span : lane;
+    value = __shfl_sync(0xffffffffu, value, from & 31);
+    key = __shfl_sync(0xffffffffu, (int)key, from & 31) && lane < a.groups ? choice_key(value, lane) : 0;
+    int above = 0;
+    for (int g = 0; g < a.groups; ++g) above += __shfl_sync(0xffffffffu, key, g) > key;
+    const bool kept = key && above < a.top_groups;
+    const unsigned open = __ballot_sync(0xffffffffu, kept);
+    // order bits of the least kept and of the best left out
+    const uint32_t low = __reduce_min_sync(0xffffffffu, kept ? (uint32_t)(key >> 32) : 0xffffffffu);
+    const uint32_t high = __reduce_max_sync(0xffffffffu, !kept && key ? (uint32_t)(key >> 32) : 0u);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int g = whole ? lane / span : (lane * a.each + i) / size;
+        if (g < 32 && !(open >> g & 1u)) k.c[i] = -INFINITY;
+    }
+    return high && open ? from_order_bits(low) - from_order_bits(high) : INFINITY;
+}
+
+// The top_k best, ties to the lower expert, the j-th in lane j. `margin`: how far two choices have
+// to be apart for their order to be sure, or 0 where they are exact; false when some two that decide
+// are nearer without being equal by their inputs (`x`, and no bias).
+template <int NS>
+__device__ __forceinline__ bool take_best(const RouteArgs& a, Choices<NS>& k, const float (&x)[NS], float margin, int lane,
+                                          int& chosen) {
+    chosen = -1;
+    float before = INFINITY, before_x = 0.f;
+    bool sure = true;
+    k.best();
+    const int rounds = margin > 0.f ? a.top_k + 1 : a.top_k;
+    for (int j = 0; j < rounds; ++j) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, k.ord);
+        if (!m) break;
+        const int e = __reduce_min_sync(0xffffffffu, k.ord == m ? lane * a.each + k.slot : 0x7fffffff);
+        const int owner = __ffs(__ballot_sync(0xffffffffu, k.ord == m && lane * a.each + k.slot == e)) - 1;
+        if (margin > 0.f) {
+            const float c = from_order_bits(m);
+            float mine = x[0];
+#pragma unroll
+            for (int i = 1; i < NS; ++i) mine = i == k.slot ? x[i] : mine;
+            const float cx = __shfl_sync(0xffffffffu, mine, owner);
+            // equal inputs are equal choices, but behind the last one others may follow that are near
+            const bool equal = cx == before_x && !a.bias && j > 0 && j < a.top_k;
+            if (!(before - c > margin + 0x1p-21f * fabsf(c)) && !equal) sure = false;
+            before = c;
+            before_x = cx;
+        }
+        if (lane == j && j < a.top_k) chosen = e;
+        if (lane == owner) {
+            k.drop(k.slot);
+            k.best();
+        }
+    }
+    return sure;
+}
+
+// A warp per row. Softmax scores are computed in 64 bits. Sigmoid scores are computed in 32 first
+// (2 units in the last place for the exponential, 2 for the quotient, the sum's rounding: 2^-20.6 of
+// the score) and where all the choices that decide are further apart than two such errors they
+// stand as they would in 64 bits; only else are all of the row's scores computed in 64. The weights
+// always come from the exact scores of the chosen.
+template <typename T, int NS, bool SIGMOID>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteArgs a) {
     extern __shared__ float route_smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = (int64_t)blockIdx.x * kRouteWarps + warp;
     if (row >= a.rows) return;
-    float* score = route_smem + warp * 2 * a.experts;
-    float* choice = score + a.experts;  // -inf: not in A, or its group was not chosen
-    const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+    const T* logits = static_cast<const T*>(a.logits) + row * a.row_stride;
+    float* const by_expert = route_smem + warp * a.experts;
 
-    double m = -INFINITY, sum = 0.0;
-    if (!a.sigmoid) {
-        for (int e = lane; e < a.experts; e += 32) {
-            const double l = fmin((double)to_f32(x[e]), (double)3.402823466e38f);  // NaN: not in A
-            const float b = a.bias ? __ldg(a.bias + e) : 0.f;
-            if (to_f32(x[e]) > -INFINITY && b > -INFINITY) m = fmax(m, l);
-        }
+    float x[NS];
+    const int e0 = lane * a.each;
+    constexpr int kVec = 16 / sizeof(T);
+    if (NS >= kVec && a.wide) {  // each == NS
+        if constexpr (NS >= kVec) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-        for (int e = lane; e < a.experts; e += 32) {
-            const double l = fmin((double)to_f32(x[e]), (double)3.402823466e38f);
-            const float b = a.bias ? __ldg(a.bias + e) : 0.f;
-            if (to_f32(x[e]) > -INFINITY && b > -INFINITY) sum += exp(l - m);
+            for (int i = 0; i < NS; i += kVec) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(logits + e0 + i));
+                T v[kVec];
+                *reinterpret_cast<uint4*>(v) = u;
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) x[i + j] = to_f32(v[j]);
+            }
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) x[i] = i < a.each && e0 + i < a.experts ? to_f32(logits[e0 + i]) : -INFINITY;
+    }
+    float b[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        b[i] = a.bias && i < a.each && e0 + i < a.experts ? __ldg(a.bias + e0 + i) : 0.f;
+        if (!(x[i] > -INFINITY && b[i] > -INFINITY)) x[i] = -INFINITY;  // NaN too
+    }
+
+    Choices<NS> k;
+    int chosen = -1;
+    double m = 0.0, sum = 1.0;
+    bool sure = false;
+    if (SIGMOID) {
+        float high = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const float s = __fdividef(1.f, 1.f + expf(fminf(-x[i], 80.f)));
+            k.c[i] = x[i] > -INFINITY ? __fadd_rn(s, b[i]) : -INFINITY;
+            if (x[i] > -INFINITY) high = fmaxf(high, s);
+        }
+        high = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high)));
+        const float margin = fmaxf(0x1p-19f * high, 4e-35f);  // e^-80 stands for all below it
+        const float gap = a.groups > 1 ? keep_groups(a, k, by_expert, lane) : INFINITY;
+        sure = take_best(a, k, x, margin, lane, chosen) && gap > 4.f * margin;
+        if (a.groups > 1 && sure) {
+            // a group's sum may be large by its bias: its own rounding counts too
+            float large = 0.f;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) large = fmaxf(large, fabsf(b[i]) < INFINITY ? fabsf(b[i]) : 0.f);
+            large = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(large)));
+            sure = gap > 4.f * margin + 0x1p-19f * large;
+        }
+    } else {
+        float high = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) high = fmaxf(high, x[i]);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, order_bits(high));
+        m = exact_logit(from_order_bits(top));
+        sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (x[i] > -INFINITY) sum += exp(exact_logit(x[i]) - m);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
-    for (int e = lane; e < a.experts; e += 32) {
-        const float l = to_f32(x[e]), b = a.bias ? __ldg(a.bias + e) : 0.f;
-        const double d = fmin((double)l, (double)3.402823466e38f);  // +inf as the largest logit
-        const bool in = l > -INFINITY && b > -INFINITY;
-        const float s = !in ? 0.f : (float)(a.sigmoid ? 1.0 / (1.0 + exp(-d)) : exp(d - m) / sum);
-        score[e] = s;
-        choice[e] = in ? __fadd_rn(s, b) : -INFINITY;
-    }
-    __syncwarp();
-    if (a.groups > 1) {
-        const int size = a.experts / a.groups;
-        uint64_t mine = 0;
-        if (lane < a.groups) {
-            float first = -INFINITY, second = -INFINITY;
-            for (int i = 0; i < size; ++i) {
-                const float c = choice[lane * size + i];
-                if (c > first) {
-                    second = first;
-                    first = c;
-                } else if (c > second) {
-                    second = c;
-                }
-            }
-            if (first > -INFINITY)
-                mine = choice_key(a.group_top2 && second > -INFINITY ? __fadd_rn(first, second) : first, lane);
+    auto exact = [&](float v) { return SIGMOID ? exact_sigmoid(v) : (float)(exp(exact_logit(v) - m) / sum); };
+    if (!sure) {  // the whole warp
+#pragma unroll
+        for (int i = 0; i < NS; ++i) k.c[i] = x[i] > -INFINITY ? __fadd_rn(exact(x[i]), b[i]) : -INFINITY;
+        if (a.groups > 1) {
+            __syncwarp();
+            keep_groups(a, k, by_expert, lane);
         }
-        int rank = 0;
-        for (int g = 0; g < a.groups; ++g) rank += __shfl_sync(0xffffffffu, mine, g) > mine;
-        if (lane < a.groups && rank >= a.top_groups)
-            for (int i = 0; i < size; ++i) choice[lane * size + i] = -INFINITY;
-        __syncwarp();
+        take_best(a, k, x, 0.f, lane, chosen);
     }
-    double total = 0.0;
-    uint64_t mine = 0, last = ~0ull;  // lane j keeps the j-th chosen
-    for (int j = 0; j < a.top_k; ++j) {
-        uint64_t k = 0;
-        for (int e = lane; e < a.experts; e += 32) {
-            if (!(choice[e] > -INFINITY)) continue;
-            const uint64_t c = choice_key(choice[e], e);
-            if (c < last && c > k) k = c;
-        }
-        k = warp_max(k);
-        if (k) total += (double)score[key_index(k)];
-        if (lane == j) mine = k;
-        last = k;
+
+    const double score = chosen >= 0 ? (double)exact(to_f32(logits[chosen])) : 0.0;
+    double w = score;
+    if (a.renormalise) {
+        double total = 0.0;
+        for (int j = 0; j < a.top_k; ++j) total += __shfl_sync(0xffffffffu, score, j);
+        w = total > 0.0 ? w / total : 0.0;
     }
     if (lane < a.top_k) {
-        const int e = mine ? key_index(mine) : -1;
-        double w = 0.0;
-        if (e >= 0) {
-            w = score[e];
-            if (a.renormalise) w = total > 0.0 ? w / total : 0.0;
-            w *= (double)a.scale;
-        }
-        a.ids[row * a.top_k + lane] = e;
-        a.weights[row * a.top_k + lane] = (float)w;
+        a.ids[row * a.top_k + lane] = chosen;
+        a.weights[row * a.top_k + lane] = (float)(w * (double)a.scale);
     }
+}
+
+template <typename T, int NS>
+void launch_route_slots(const RouteArgs& a, bool sigmoid, cudaStream_t stream) {
+    const unsigned ctas = (unsigned)(((int64_t)a.rows + kRouteWarps - 1) / kRouteWarps);
+    const int smem = a.groups > 1 && a.experts / a.groups % a.each ? kRouteWarps * a.experts * (int)sizeof(float) : 0;
+    if (sigmoid) route_kernel<T, NS, true><<<ctas, kRouteThreads, smem, stream>>>(a);
+    else route_kernel<T, NS, false><<<ctas, kRouteThreads, smem, stream>>>(a);
+}
+
+template <typename T>
+void launch_route_type(RouteArgs a, bool sigmoid, cudaStream_t stream) {
+    a.each = (a.experts + 31) / 32;
+    int ns = 1;
+    while (ns < a.each) ns *= 2;
+    a.wide = a.each == ns && a.experts == 32 * ns && ns * sizeof(T) >= 16 &&
+             (reinterpret_cast<uintptr_t>(a.logits) | (uintptr_t)(a.row_stride * (int64_t)sizeof(T))) % 16 == 0;
+    if (ns == 1) launch_route_slots<T, 1>(a, sigmoid, stream);
+    else if (ns == 2) launch_route_slots<T, 2>(a, sigmoid, stream);
+    else if (ns == 4) launch_route_slots<T, 4>(a, sigmoid, stream);
+    else if (ns == 8) launch_route_slots<T, 8>(a, sigmoid, stream);
+    else if (ns == 16) launch_route_slots<T, 16>(a, sigmoid, stream);
+    else launch_route_slots<T, 32>(a, sigmoid, stream);
 }
 
 // ---- plan -----------------------------------------------------------------------------------
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanCluster = 8;
+constexpr int kPlanAhead = 4;  // ids a lane has in flight
 
 struct PlanArgs {
     const int32_t* ids;
@@ -145,35 +301,65 @@ struct PlanArgs {
     int32_t* offsets;
 };
 
-// One CTA. Each warp owns a run of assignments and a row of counters: it counts its run's experts,
-// the counters become the places before which this warp's assignments of each expert go, and it
-// walks its run again in order, so that the sort is stable and no atomic decides a place.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanArgs a) {
-    extern __shared__ int plan_smem[];  // [kPlanWarps][experts]
-    __shared__ int scan[kPlanWarps];
+// One CTA, or one cluster of them. Each warp owns a run of assignments and a row of counters: it
+// counts its run's experts, the counters become the places before which this warp's assignments
+// of each expert go (after those of earlier warps, earlier CTAs and lower experts), and it walks its
+// run again in order, so that the sort is stable and no atomic decides a place.
+__global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ PlanArgs a) {
+    extern __shared__ int plan_smem[];
+    __shared__ int scan[32];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int threads = blockDim.x, warps = threads / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int* mine = plan_smem + warp * a.experts;
+    int* const totals = plan_smem;             // [experts] of this CTA, read by the others
+    int* const base = totals + a.experts;      // [experts]
+    int* const counts = base + a.experts;      // [warps][experts]
+    int* const mine = counts + warp * a.experts;
     for (int e = lane; e < a.experts; e += 32) mine[e] = 0;
     __syncwarp();
-    const int64_t run = ((((int64_t)a.pairs + kPlanWarps - 1) / kPlanWarps) + 31) & ~(int64_t)31;
-    const int64_t lo = min((int64_t)a.pairs, run * warp), hi = min((int64_t)a.pairs, lo + run);
-    for (int64_t i = lo + lane; i - lane < hi; i += 32) {
-        int id = i < hi ? a.ids[i] : -1;
-        if (id < 0 || id >= a.experts) id = -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, id);
-        if (id >= 0 && lane == __ffs(peers) - 1) mine[id] += __popc(peers);
-        __syncwarp();
+    const int64_t run = (((int64_t)a.pairs + ranks * warps - 1) / (ranks * warps) + 31) & ~(int64_t)31;
+    const int lo = (int)min((int64_t)a.pairs, run * (rank * warps + warp)), hi = (int)min((int64_t)a.pairs, lo + run);
+    auto read = [&](int i) {
+        const int id = i < hi ? __ldg(a.ids + i) : -1;
+        return id >= 0 && id < a.experts ? id : -1;
+    };
+    for (int i0 = lo; i0 < hi; i0 += 32 * kPlanAhead) {
+        int id[kPlanAhead];
+#pragma unroll
+        for (int q = 0; q < kPlanAhead; ++q) id[q] = read(i0 + 32 * q + lane);
+#pragma unroll
+        for (int q = 0; q < kPlanAhead; ++q)
+            if (id[q] >= 0) atomicAdd(mine + id[q], 1);
     }
     __syncthreads();
-    int total = 0;
-    if (tid < a.experts) {
-        for (int w = 0; w < kPlanWarps; ++w) {
-            const int c = plan_smem[w * a.experts + tid];
-            plan_smem[w * a.experts + tid] = total;
+    for (int e = tid; e < a.experts; e += threads) {
+        int total = 0;
+        for (int w = 0; w < warps; ++w) {
+            const int c = counts[w * a.experts + e];
+            counts[w * a.experts + e] = total;
             total += c;
         }
+        totals[e] = total;
     }
-    int incl = total;
+    // every expert's count over the CTAs, and over those before this one; a thread has a run of experts
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+    const int each = (a.experts + threads - 1) / threads;
+    const int e0 = min(a.experts, tid * each), e1 = min(a.experts, e0 + each);
+    int sum = 0;
+    for (int e = e0; e < e1; ++e) {
+        int before = 0, all = 0;
+        for (int r = 0; r < ranks; ++r) {
+            const int c = ranks > 1 ? *cluster.map_shared_rank(totals + e, r) : totals[e];
+            before += r < rank ? c : 0;
+            all += c;
+        }
+        base[e] = sum + before;
+        sum += all;
+    }
+    if (ranks > 1) cluster.barrier_arrive();  // the others' totals have been read
+    int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -181,35 +367,42 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    int before = 0, kept = 0;
-    for (int w = 0; w < kPlanWarps; ++w) {
-        if (w < warp) before += scan[w];
+    int first = incl - sum, kept = 0;
+    for (int w = 0; w < warps; ++w) {
+        first += w < warp ? scan[w] : 0;
         kept += scan[w];
     }
-    const int first = before + incl - total;
-    if (tid < a.experts) {
-        a.offsets[tid] = first;
-        for (int w = 0; w < kPlanWarps; ++w) plan_smem[w * a.experts + tid] += first;
+    for (int e = e0; e < e1; ++e) {
+        base[e] += first;
+        if (rank == 0) a.offsets[e] = base[e];  // nothing comes before the first CTA's
     }
-    if (tid == 0) a.offsets[a.experts] = kept;
+    if (rank == 0 && tid == 0) a.offsets[a.experts] = kept;
     __syncthreads();
-    for (int64_t i = lo + lane; i - lane < hi; i += 32) {
-        int id = i < hi ? a.ids[i] : -1;
-        if (id < 0 || id >= a.experts) id = -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, id);
-        const int place = id >= 0 ? mine[id] + __popc(peers & ((1u << lane) - 1u)) : -1;
-        __syncwarp();
-        if (id >= 0 && lane == __ffs(peers) - 1) mine[id] += __popc(peers);
-        __syncwarp();
-        if (i < hi) a.slots[i] = place;
-        if (place >= 0) a.order[place] = (int)(i / a.k);
+    for (int i0 = lo; i0 < hi; i0 += 32 * kPlanAhead) {
+        int id[kPlanAhead];
+#pragma unroll
+        for (int q = 0; q < kPlanAhead; ++q) id[q] = read(i0 + 32 * q + lane);
+#pragma unroll
+        for (int q = 0; q < kPlanAhead; ++q) {
+            const int i = i0 + 32 * q + lane;
+            const unsigned peers = __match_any_sync(0xffffffffu, id[q]);
+            int place = -1;
+            if (id[q] >= 0) place = base[id[q]] + mine[id[q]] + __popc(peers & ((1u << lane) - 1u));
+            __syncwarp();
+            if (id[q] >= 0 && lane == __ffs(peers) - 1) mine[id[q]] += __popc(peers);
+            __syncwarp();
+            if (i < hi) a.slots[i] = place;
+            if (place >= 0) a.order[place] = (int)((unsigned)i / (unsigned)a.k);
+        }
     }
-    for (int64_t i = (int64_t)kept + tid; i < a.pairs; i += kPlanThreads) a.order[i] = -1;
+    for (int64_t i = (int64_t)kept + rank * threads + tid; i < a.pairs; i += ranks * threads) a.order[i] = -1;
+    if (ranks > 1) cluster.barrier_wait();  // no CTA leaves while its totals are read
 }
 
 // ---- combine --------------------------------------------------------------------------------
 
 constexpr int kCombineThreads = 256;
+constexpr int kCombineAhead = 8;  // results a thread has in flight
 
 struct CombineArgs {
     const void* rows;
@@ -218,21 +411,73 @@ struct CombineArgs {
     const float* weights;
     const int32_t* slots;
     int n, k, width;
+    int per_cta;  // rows of a CTA
     void* out;
 };
 
-template <typename T>
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T)) Pack {
+    T v[VEC];
+};
+
+// A thread per row and VEC adjacent columns. Bound by memory: each result is read once.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ CombineArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * kCombineThreads + threadIdx.x;
-    if (i >= (int64_t)a.n * a.width) return;
-    const int64_t row = i / a.width, c = i - row * a.width;
-    float sum = 0.f;
-    for (int j = 0; j < a.k; ++j) {
-        const int slot = __ldg(a.slots + row * a.k + j);
-        if (slot < 0 || slot >= a.n_rows) continue;
-        sum = __fmaf_rn(__ldg(a.weights + row * a.k + j), to_f32(static_cast<const T*>(a.rows)[slot * a.row_stride + c]), sum);
+    using P = Pack<T, VEC>;
+    const unsigned cols = (unsigned)(a.width / VEC);
+    const unsigned in_cta = a.per_cta > 1 ? threadIdx.x / cols : 0;
+    const int64_t row = (int64_t)blockIdx.x * a.per_cta + in_cta;
+    if (in_cta >= (unsigned)a.per_cta || row >= a.n) return;
+    const float* weights = a.weights + row * a.k;
+    const int32_t* slots = a.slots + row * a.k;
+    for (unsigned c = a.per_cta > 1 ? threadIdx.x - in_cta * cols : blockIdx.y * kCombineThreads + threadIdx.x; c < cols;
+         c += gridDim.y * kCombineThreads) {
+        float sum[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+        for (int j0 = 0; j0 < a.k; j0 += kCombineAhead) {
+            P p[kCombineAhead];
+            float w[kCombineAhead];
+#pragma unroll
+            for (int j = 0; j < kCombineAhead; ++j) {
+                const int slot = j0 + j < a.k ? __ldg(slots + j0 + j) : -1;
+                w[j] = 0.f;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) from_f32(0.f, &p[j].v[i]);
+                if (slot >= 0 && slot < a.n_rows) {
+                    w[j] = __ldg(weights + j0 + j);
+                    p[j] = *reinterpret_cast<const P*>(static_cast<const T*>(a.rows) + slot * a.row_stride + (int64_t)c * VEC);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kCombineAhead; ++j)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) sum[i] = __fmaf_rn(w[j], to_f32(p[j].v[i]), sum[i]);
+        }
+        P out;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) from_f32(sum[i], &out.v[i]);
+        *reinterpret_cast<P*>(static_cast<T*>(a.out) + row * a.width + (int64_t)c * VEC) = out;
     }
-    from_f32(sum, static_cast<T*>(a.out) + i);
+}
+
+template <typename T, int VEC>
+void launch_combine_vec(CombineArgs a, cudaStream_t stream) {
+    const int64_t cols = a.width / VEC;
+    a.per_cta = cols < kCombineThreads ? (int)(kCombineThreads / cols) : 1;
+    const dim3 grid((unsigned)(((int64_t)a.n + a.per_cta - 1) / a.per_cta),
+                    (unsigned)std::min<int64_t>((cols + kCombineThreads - 1) / kCombineThreads, 65535));
+    combine_kernel<T, VEC><<<grid, kCombineThreads, 0, stream>>>(a);
+}
+
+// The widest loads that every row's start, in and out, allows.
+template <typename T>
+void launch_combine_type(const CombineArgs& a, cudaStream_t stream) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.rows) | reinterpret_cast<uintptr_t>(a.out) |
+                         (uintptr_t)(a.row_stride * (int64_t)sizeof(T)) | (uintptr_t)((int64_t)a.width * sizeof(T));
+    if (at % 16 == 0) launch_combine_vec<T, 16 / sizeof(T)>(a, stream);
+    else if (sizeof(T) == 2 && at % 4 == 0) launch_combine_vec<T, sizeof(T) == 2 ? 2 : 1>(a, stream);
+    else launch_combine_vec<T, 1>(a, stream);
 }
 
 Status launched() {
@@ -245,34 +490,44 @@ Status launched() {
 Status launch_route(const void* logits, int dtype, int rows, int experts, int64_t row_stride, const float* bias,
                     int top_k, int sigmoid, int groups, int top_groups, int group_top2, int renormalise, float scale,
                     float* weights, int32_t* ids, cudaStream_t stream) {
-    const RouteArgs a{logits, rows, experts, row_stride, bias, top_k, sigmoid, groups,
-                      top_groups, group_top2, renormalise, scale, weights, ids};
-    const int ctas = (int)(((int64_t)rows + kRouteWarps - 1) / kRouteWarps);
-    const int smem = kRouteWarps * 2 * experts * (int)sizeof(float);  // at most 32 KB
-    if (dtype == SHIPK_DTYPE_F32) route_kernel<float><<<ctas, kRouteThreads, smem, stream>>>(a);
-    else if (dtype == SHIPK_DTYPE_F16) route_kernel<__half><<<ctas, kRouteThreads, smem, stream>>>(a);
-    else route_kernel<__nv_bfloat16><<<ctas, kRouteThreads, smem, stream>>>(a);
+    const RouteArgs a{logits, rows, experts, row_stride, bias, top_k, groups, top_groups, group_top2,
+                      renormalise, 0, 0, scale, weights, ids};
+    if (dtype == SHIPK_DTYPE_F32) launch_route_type<float>(a, sigmoid, stream);
+    else if (dtype == SHIPK_DTYPE_F16) launch_route_type<__half>(a, sigmoid, stream);
+    else launch_route_type<__nv_bfloat16>(a, sigmoid, stream);
     return launched();
 }
 
 Status launch_plan(const int32_t* ids, int rows, int k, int experts, int32_t* order, int32_t* slots, int32_t* offsets,
                    cudaStream_t stream) {
     const PlanArgs a{ids, rows * k, k, experts, order, slots, offsets};
-    const int smem = kPlanWarps * experts * (int)sizeof(int);
-    const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(plan_kernel), kPlanWarps * kMaxExperts * (int)sizeof(int));
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(plan_kernel), (2 + 32) * kMaxExperts * (int)sizeof(int));
     if (e != cudaSuccess) return Status{SHIPK_ECUDA, cudaGetErrorString(e)};
-    plan_kernel<<<1, kPlanThreads, smem, stream>>>(a);
-    return launched();
+    // a cluster once a CTA's warps would walk for long; a warp for every 128 assignments
+    const int ranks = a.pairs > 8192 ? kPlanCluster : 1;
+    const int64_t warps = ((int64_t)a.pairs / ranks + 127) / 128;
+    const int threads = 32 * (int)std::min<int64_t>(std::max<int64_t>(warps, 4), 32);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)ranks);
+    config.blockDim = dim3((unsigned)threads);
+    config.dynamicSmemBytes = (size_t)(2 + threads / 32) * experts * sizeof(int);
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)ranks, 1, 1};
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    e = cudaLaunchKernelEx(&config, plan_kernel, a);
+    const Status s = launched();
+    return e == cudaSuccess ? s : Status{SHIPK_ECUDA, cudaGetErrorString(e)};
 }
 
 Status launch_combine(const void* in, int dtype, int n_in, int64_t row_stride, const float* weights, const int32_t* slots,
                       int rows, int k, int width, void* out, cudaStream_t stream) {
-    const CombineArgs a{in, n_in, row_stride, weights, slots, rows, k, width, out};
-    const int64_t ctas = ((int64_t)rows * width + kCombineThreads - 1) / kCombineThreads;
-    if (ctas > 0x7fffffff) return Status{SHIPK_ERANGE, "more than 2^39 output values"};
-    if (dtype == SHIPK_DTYPE_F32) combine_kernel<float><<<(int)ctas, kCombineThreads, 0, stream>>>(a);
-    else if (dtype == SHIPK_DTYPE_F16) combine_kernel<__half><<<(int)ctas, kCombineThreads, 0, stream>>>(a);
-    else combine_kernel<__nv_bfloat16><<<(int)ctas, kCombineThreads, 0, stream>>>(a);
+    const CombineArgs a{in, n_in, row_stride, weights, slots, rows, k, width, 1, out};
+    if (dtype == SHIPK_DTYPE_F32) launch_combine_type<float>(a, stream);
+    else if (dtype == SHIPK_DTYPE_F16) launch_combine_type<__half>(a, stream);
+    else launch_combine_type<__nv_bfloat16>(a, stream);
     return launched();
 }
 

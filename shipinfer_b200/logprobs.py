@@ -11,6 +11,8 @@ from __future__ import annotations
 
 from typing import Any
 
+import torch
+
 from shipinfer_b200 import _native
 from shipinfer_b200._heads import check_dense, check_device, check_matrix, element_code, empty, guard, handle_of, ptr, small
 from shipinfer_b200.errors import ValidationError
@@ -21,8 +23,6 @@ __all__ = ["pack_allowed", "token_logprobs_device"]
 def pack_allowed(mask: Any) -> Any:
     """A bool mask ``[vocab]`` or ``[rows, vocab]`` as the bits :func:`token_logprobs_device`
     reads: int32 ``[words]`` or ``[rows, words]``, token ``v`` in bit ``v % 32`` of word ``v // 32``."""
-    import torch
-
     if mask.dtype != torch.bool or mask.dim() not in (1, 2):
         raise ValidationError(f"mask must be a bool [vocab] or [rows, vocab] tensor; got {mask.dtype} {list(mask.shape)}")
     vocab = int(mask.shape[-1])
@@ -66,8 +66,6 @@ def token_logprobs_device(
         alternative id -1 and -inf. A row with nothing allowed has -inf, entropy 0 and no
         alternatives; a NaN or +inf among the allowed scores makes its numbers NaN.
     """
-    import torch
-
     rows, vocab = check_matrix(logits, "logits")
     code = element_code(logits, "logits")
     top = small(top, "top")
@@ -99,7 +97,7 @@ def token_logprobs_device(
         check_dense(top_logprobs, "top_logprobs", torch.float32, (rows, top))
     if top_ids is not None:
         check_dense(top_ids, "top_ids", torch.int64, (rows, top))
-    dev = check_device(logits, logits=logits, tokens=tokens, allowed=allowed, logprobs=logprobs, entropy=entropy,
+    dev = check_device(logits, tokens=tokens, allowed=allowed, logprobs=logprobs, entropy=entropy,
                        top_logprobs=top_logprobs, top_ids=top_ids)
     if logprobs is None:
         logprobs = empty(shape, torch.float32, dev, stream)

@@ -17,6 +17,8 @@ from __future__ import annotations
 
 from typing import Any
 
+import torch
+
 from shipinfer_b200 import _native
 from shipinfer_b200._heads import check_dense, check_device, check_matrix, element_code, empty, guard, handle_of, ptr, small
 from shipinfer_b200.errors import ValidationError
@@ -64,8 +66,6 @@ def route_experts_device(
         expert that can be chosen, id -1 and weight 0. The scores are computed in 64 bits and
         rounded once, so the choice does not depend on how a sum was ordered.
     """
-    import torch
-
     rows, experts = check_matrix(logits, "logits")
     code = element_code(logits, "logits")
     top_k, groups, top_groups = small(top_k, "top_k"), small(groups, "groups"), small(top_groups, "top_groups")
@@ -79,7 +79,7 @@ def route_experts_device(
         check_dense(weights, "weights", torch.float32, (rows, top_k))
     if ids is not None:
         check_dense(ids, "ids", torch.int32, (rows, top_k))
-    dev = check_device(logits, logits=logits, bias=bias, weights=weights, ids=ids)
+    dev = check_device(logits, bias=bias, weights=weights, ids=ids)
     if weights is None:
         weights = empty((rows, max(top_k, 0)), torch.float32, dev, stream)
     if ids is None:
@@ -119,8 +119,6 @@ def plan_experts_device(
         ``order[offsets[e]:offsets[e + 1]]``, ascending; places past ``offsets[experts]`` hold -1.
         ``slots[r, j]`` is the place of row r's j-th expert, -1 where there is none.
     """
-    import torch
-
     if ids.dim() != 2:
         raise ValidationError(f"ids must be int32 [rows, k]; got {list(ids.shape)}")
     rows, k = small(ids.shape[0], "rows"), small(ids.shape[1], "k")
@@ -132,7 +130,7 @@ def plan_experts_device(
         check_dense(slots, "slots", torch.int32, (rows, k))
     if offsets is not None:
         check_dense(offsets, "offsets", torch.int32, (experts + 1,))
-    dev = check_device(ids, ids=ids, order=order, slots=slots, offsets=offsets)
+    dev = check_device(ids, order=order, slots=slots, offsets=offsets)
     if order is None:
         order = empty((rows * k,), torch.int32, dev, stream)
     if slots is None:
@@ -168,8 +166,6 @@ def combine_experts_device(
     Returns:
         ``[r, width]`` on the device, summed in 32 bits in the order of j and rounded once.
     """
-    import torch
-
     n, width = check_matrix(rows, "rows")
     code = element_code(rows, "rows")
     if slots.dim() != 2:
@@ -179,7 +175,7 @@ def combine_experts_device(
     check_dense(weights, "weights", torch.float32, (r, k))
     if out is not None:
         check_dense(out, "out", rows.dtype, (r, width))
-    dev = check_device(slots, slots=slots, weights=weights, rows=rows, out=out)
+    dev = check_device(slots, weights=weights, rows=rows, out=out)
     if out is None:
         out = empty((r, width), rows.dtype, dev, stream)
     with guard(dev):
