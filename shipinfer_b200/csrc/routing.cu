@@ -38,7 +38,7 @@ struct RouteArgs {
     const float* bias;
     int top_k, groups, top_groups, group_top2, renormalise;
     int each;  // experts of a lane
-    int wide;  // 16 bytes of a lane's logits at a time
+    int wide, wide_bias;  // a lane's logits, and its biases, 16 bytes at a time
     float scale;
     float* weights;
     int32_t* ids;
@@ -52,25 +52,21 @@ __device__ __forceinline__ float exact_sigmoid(float x) { return (float)(1.0 / (
 template <int NS>
 struct Choices {
     float c[NS];
-    uint32_t ord;  // the lane's best: its order bits (0: none) and its slot
-    int slot;
 
-    __device__ __forceinline__ void best() {
+    __device__ __forceinline__ float best() const {
         float m = c[0];
-        slot = 0;
 #pragma unroll
-        for (int i = 1; i < NS; ++i)
-            if (c[i] > m) {
-                m = c[i];
-                slot = i;
-            }
-        ord = m > -INFINITY ? order_bits(m) : 0u;
+        for (int i = 1; i < NS; ++i) m = fmaxf(m, c[i]);
+        return m;
     }
-    __device__ __forceinline__ void drop(int s) {
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-            if (i == s) c[i] = -INFINITY;
-    }
+};
+
+// Shared by a warp: the choices that reach a bound, in any order.
+constexpr int kListed = 64;
+struct Listed {
+    uint64_t keys[kListed];
+    float x[kListed];       // their logits
+    int8_t order[kListed];  // the entry of each rank
 };
 
 // The larger two of two descending pairs.
@@ -130,39 +126,82 @@ __device__ __forceinline__ float keep_groups(const RouteArgs& a, Choices<NS>& k,
 
 // The top_k best, ties to the lower expert, the j-th in lane j. `margin`: how far two choices have
 // to be apart for their order to be sure, or 0 where they are exact; false when some two that decide
-// are nearer without being equal by their inputs (`x`, and no bias).
+// are nearer without being equal by their inputs (the logit, and no bias).
+//
+// The top_k-th largest of the lanes' maxima bounds the choices: at least top_k reach it, and few
+// more. Those that do (or come within the margin of it) are listed and ranked. More than the list holds,
+// by ties or many of them: taken one at a time.
 template <int NS>
 __device__ __forceinline__ bool take_best(const RouteArgs& a, Choices<NS>& k, const float (&x)[NS], float margin, int lane,
-                                          int& chosen) {
-    chosen = -1;
-    float before = INFINITY, before_x = 0.f;
-    bool sure = true;
-    k.best();
-    const int rounds = margin > 0.f ? a.top_k + 1 : a.top_k;
-    for (int j = 0; j < rounds; ++j) {
-        const uint32_t m = __reduce_max_sync(0xffffffffu, k.ord);
-        if (!m) break;
-        const int e = __reduce_min_sync(0xffffffffu, k.ord == m ? lane * a.each + k.slot : 0x7fffffff);
-        const int owner = __ffs(__ballot_sync(0xffffffffu, k.ord == m && lane * a.each + k.slot == e)) - 1;
-        if (margin > 0.f) {
-            const float c = from_order_bits(m);
-            float mine = x[0];
-#pragma unroll
-            for (int i = 1; i < NS; ++i) mine = i == k.slot ? x[i] : mine;
-            const float cx = __shfl_sync(0xffffffffu, mine, owner);
-            // equal inputs are equal choices, but behind the last one others may follow that are near
-            const bool equal = cx == before_x && !a.bias && j > 0 && j < a.top_k;
-            if (!(before - c > margin + 0x1p-21f * fabsf(c)) && !equal) sure = false;
-            before = c;
-            before_x = cx;
-        }
-        if (lane == j && j < a.top_k) chosen = e;
-        if (lane == owner) {
-            k.drop(k.slot);
-            k.best();
-        }
+                                          Listed& list, int& chosen) {
+    const float m = k.best();
+    const uint32_t mine = m > -INFINITY ? order_bits(m) : 0u;
+    uint32_t left = mine, t = 0;
+    for (int j = 0; j < a.top_k; ++j) {
+        t = __reduce_max_sync(0xffffffffu, left);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, left == t)) - 1) left = 0;
     }
-    return sure;
+    float least = t ? from_order_bits(t) : -INFINITY;
+    if (margin > 0.f) least = least - (margin + 0x1p-21f * fabsf(least));  // NaN, which nothing reaches, for +inf
+    int n = 0;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const bool in = k.c[i] >= least && k.c[i] > -INFINITY;
+        const unsigned who = __ballot_sync(0xffffffffu, in);
+        const int at = n + __popc(who & ((1u << lane) - 1u));
+        if (in && at < kListed) {
+            list.keys[at] = choice_key(k.c[i], lane * a.each + i);
+            list.x[at] = x[i];
+        }
+        n += __popc(who);
+    }
+    __syncwarp();
+    chosen = -1;
+    if (n <= kListed) {
+        const uint64_t k0 = lane < n ? list.keys[lane] : 0, k1 = lane + 32 < n ? list.keys[lane + 32] : 0;
+        int r0 = 0, r1 = 0;
+        for (int q = 0; q < n; ++q) {
+            const uint64_t other = list.keys[q];
+            r0 += other > k0;
+            r1 += other > k1;
+        }
+        if (lane < n) list.order[r0] = (int8_t)lane;
+        if (lane + 32 < n) list.order[r1] = (int8_t)(lane + 32);
+        __syncwarp();
+        if (lane < min(n, a.top_k)) chosen = key_index(list.keys[list.order[lane]]);
+        if (margin > 0.f) {
+            // each choice against the one behind it; what is not listed is further than the margin.
+            // Equal inputs are equal choices, but behind the last one others may follow that are near.
+            if (!(least > -INFINITY) && t) return false;
+            bool sure = true;
+            if (lane < min(n - 1, a.top_k)) {
+                const int u = list.order[lane], v = list.order[lane + 1];
+                const float hi = key_value(list.keys[u]), lo = key_value(list.keys[v]);
+                const bool equal = list.x[u] == list.x[v] && !a.bias && lane + 1 < a.top_k;
+                sure = hi - lo > margin + 0x1p-21f * fabsf(lo) || equal;
+            }
+            return __all_sync(0xffffffffu, sure);
+        }
+        return true;
+    }
+    if (margin > 0.f) return false;
+    uint32_t o = mine;
+    for (int j = 0; j < a.top_k; ++j) {
+        const uint32_t high = __reduce_max_sync(0xffffffffu, o);
+        if (!high) break;
+        int slot = 0;
+#pragma unroll
+        for (int i = NS - 1; i >= 0; --i) slot = k.c[i] > -INFINITY && order_bits(k.c[i]) == o ? i : slot;
+        const int e = __reduce_min_sync(0xffffffffu, o == high ? lane * a.each + slot : 0x7fffffff);
+        if (lane == j) chosen = e;
+        const bool own = o == high && lane * a.each + slot == e;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) k.c[i] = own && i == slot ? -INFINITY : k.c[i];
+        const float next = k.best();
+        o = next > -INFINITY ? order_bits(next) : 0u;
+    }
+    return true;
 }
 
 // A warp per row. Softmax scores are computed in 64 bits. Sigmoid scores are computed in 32 first
@@ -173,9 +212,11 @@ __device__ __forceinline__ bool take_best(const RouteArgs& a, Choices<NS>& k, co
 template <typename T, int NS, bool SIGMOID>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteArgs a) {
     extern __shared__ float route_smem[];
+    __shared__ Listed lists[kRouteWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = (int64_t)blockIdx.x * kRouteWarps + warp;
     if (row >= a.rows) return;
+    Listed& list = lists[warp];
     const T* logits = static_cast<const T*>(a.logits) + row * a.row_stride;
     float* const by_expert = route_smem + warp * a.experts;
 
@@ -199,10 +240,24 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
     }
     float b[NS];
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        b[i] = a.bias && i < a.each && e0 + i < a.experts ? __ldg(a.bias + e0 + i) : 0.f;
-        if (!(x[i] > -INFINITY && b[i] > -INFINITY)) x[i] = -INFINITY;  // NaN too
+    for (int i = 0; i < NS; ++i) b[i] = 0.f;
+    if (a.bias) {
+        if (NS >= 4 && a.wide_bias) {  // each == NS
+#pragma unroll
+            for (int i = 0; i + 3 < NS; i += 4) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(a.bias + e0 + i));
+                b[i] = v.x;
+                b[i + 1] = v.y;
+                b[i + 2] = v.z;
+                b[i + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) b[i] = i < a.each && e0 + i < a.experts ? __ldg(a.bias + e0 + i) : 0.f;
+        }
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) x[i] = x[i] > -INFINITY && b[i] > -INFINITY ? x[i] : -INFINITY;  // NaN too
 
     Choices<NS> k;
     int chosen = -1;
@@ -219,7 +274,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
         high = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high)));
         const float margin = fmaxf(0x1p-19f * high, 4e-35f);  // e^-80 stands for all below it
         const float gap = a.groups > 1 ? keep_groups(a, k, by_expert, lane) : INFINITY;
-        sure = take_best(a, k, x, margin, lane, chosen) && gap > 4.f * margin;
+        sure = take_best(a, k, x, margin, lane, list, chosen) && gap > 4.f * margin;
         if (a.groups > 1 && sure) {
             // a group's sum may be large by its bias: its own rounding counts too
             float large = 0.f;
@@ -249,7 +304,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
             __syncwarp();
             keep_groups(a, k, by_expert, lane);
         }
-        take_best(a, k, x, 0.f, lane, chosen);
+        take_best(a, k, x, 0.f, lane, list, chosen);
     }
 
     const double score = chosen >= 0 ? (double)exact(to_f32(logits[chosen])) : 0.0;
@@ -280,6 +335,7 @@ void launch_route_type(RouteArgs a, bool sigmoid, cudaStream_t stream) {
     while (ns < a.each) ns *= 2;
     a.wide = a.each == ns && a.experts == 32 * ns && ns * sizeof(T) >= 16 &&
              (reinterpret_cast<uintptr_t>(a.logits) | (uintptr_t)(a.row_stride * (int64_t)sizeof(T))) % 16 == 0;
+    a.wide_bias = a.each == ns && a.experts == 32 * ns && ns >= 4 && reinterpret_cast<uintptr_t>(a.bias) % 16 == 0;
     if (ns == 1) launch_route_slots<T, 1>(a, sigmoid, stream);
     else if (ns == 2) launch_route_slots<T, 2>(a, sigmoid, stream);
     else if (ns == 4) launch_route_slots<T, 4>(a, sigmoid, stream);
@@ -491,7 +547,7 @@ Status launch_route(const void* logits, int dtype, int rows, int experts, int64_
                     int top_k, int sigmoid, int groups, int top_groups, int group_top2, int renormalise, float scale,
                     float* weights, int32_t* ids, cudaStream_t stream) {
     const RouteArgs a{logits, rows, experts, row_stride, bias, top_k, groups, top_groups, group_top2,
-                      renormalise, 0, 0, scale, weights, ids};
+                      renormalise, 0, 0, 0, scale, weights, ids};
     if (dtype == SHIPK_DTYPE_F32) launch_route_type<float>(a, sigmoid, stream);
     else if (dtype == SHIPK_DTYPE_F16) launch_route_type<__half>(a, sigmoid, stream);
     else launch_route_type<__nv_bfloat16>(a, sigmoid, stream);
