@@ -19,6 +19,8 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <map>
+#include <mutex>
 
 namespace cg = cooperative_groups;
 
@@ -38,6 +40,7 @@ struct RouteArgs {
     const float* bias;
     int top_k, groups, top_groups, group_top2, renormalise;
     int each;  // experts of a lane
+    int size, span;  // experts of a group; its lanes, 0 where groups share lanes
     int wide, wide_bias;  // a lane's logits, and its biases, 16 bytes at a time
     float scale;
     float* weights;
@@ -80,13 +83,14 @@ __device__ __forceinline__ void merge2(float& first, float& second, float f, flo
 // group kept is above the next one.
 template <int NS>
 __device__ __forceinline__ float keep_groups(const RouteArgs& a, Choices<NS>& k, float* row, int lane) {
-    const int size = a.experts / a.groups;
-    float first = -INFINITY, second = -INFINITY;
-    const bool whole = size % a.each == 0;
-    const int span = whole ? size / a.each : 1;  // lanes of a group
-    if (whole) {
+    float first = k.c[0], second = -INFINITY;
+    const int span = a.span;
+    if (span) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) merge2(first, second, k.c[i], -INFINITY);
+        for (int i = 1; i < NS; ++i) {
+            second = fmaxf(second, fminf(first, k.c[i]));
+            first = fmaxf(first, k.c[i]);
+        }
         if ((span & (span - 1)) == 0) {
             for (int o = 1; o < span; o *= 2)
                 merge2(first, second, __shfl_xor_sync(0xffffffffu, first, o), __shfl_xor_sync(0xffffffffu, second, o));
@@ -100,26 +104,36 @@ __device__ __forceinline__ float keep_groups(const RouteArgs& a, Choices<NS>& k,
         for (int i = 0; i < NS; ++i)
             if (i < a.each && lane * a.each + i < a.experts) row[lane * a.each + i] = k.c[i];
         __syncwarp();
+        first = -INFINITY;
         if (lane < a.groups)
-            for (int i = 0; i < size; ++i) merge2(first, second, row[lane * size + i], -INFINITY);
+            for (int i = 0; i < a.size; ++i) merge2(first, second, row[lane * a.size + i], -INFINITY);
     }
-    // lane g takes group g's score as a key; 0: nothing in it can be chosen
-    float value = a.group_top2 && second > -INFINITY ? __fadd_rn(first, second) : first;
-    uint64_t key = first > -INFINITY ? 1 : 0;
-    const int from = whole ? lane * span : lane;
-    value = __shfl_sync(0xffffffffu, value, from & 31);
-    key = __shfl_sync(0xffffffffu, (int)key, from & 31) && lane < a.groups ? choice_key(value, lane) : 0;
+    // lane g takes group g's score; 0: nothing in it can be chosen
+    const float value = a.group_top2 && second > -INFINITY ? __fadd_rn(first, second) : first;
+    uint32_t ord = first > -INFINITY ? order_bits(value) : 0u;
+    if (span) ord = __shfl_sync(0xffffffffu, ord, (lane * span) & 31);
+    if (lane >= a.groups) ord = 0;
     int above = 0;
-    for (int g = 0; g < a.groups; ++g) above += __shfl_sync(0xffffffffu, key, g) > key;
-    const bool kept = key && above < a.top_groups;
+    for (int g = 0; g < a.groups; ++g) {
+        const uint32_t other = __shfl_sync(0xffffffffu, ord, g);
+        above += other > ord || (other == ord && g < lane);
+    }
+    const bool kept = ord && above < a.top_groups;
     const unsigned open = __ballot_sync(0xffffffffu, kept);
-    // order bits of the least kept and of the best left out
-    const uint32_t low = __reduce_min_sync(0xffffffffu, kept ? (uint32_t)(key >> 32) : 0xffffffffu);
-    const uint32_t high = __reduce_max_sync(0xffffffffu, !kept && key ? (uint32_t)(key >> 32) : 0u);
+    // the least kept and the best left out
+    const uint32_t low = __reduce_min_sync(0xffffffffu, kept ? ord : 0xffffffffu);
+    const uint32_t high = __reduce_max_sync(0xffffffffu, kept ? 0u : ord);
+    if (span) {
+        const int g = lane / span;
+        if (!(open >> g & 1u))
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const int g = whole ? lane / span : (lane * a.each + i) / size;
-        if (g < 32 && !(open >> g & 1u)) k.c[i] = -INFINITY;
+            for (int i = 0; i < NS; ++i) k.c[i] = -INFINITY;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int g = (lane * a.each + i) / a.size;
+            if (g < 32 && !(open >> g & 1u)) k.c[i] = -INFINITY;
+        }
     }
     return high && open ? from_order_bits(low) - from_order_bits(high) : INFINITY;
 }
@@ -261,7 +275,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
 
     Choices<NS> k;
     int chosen = -1;
-    double m = 0.0, sum = 1.0;
+    double m = 0.0, inv = 1.0;
+    double e[SIGMOID || NS > 8 ? 1 : NS];  // more would cost the warps that hide the exponentials
     bool sure = false;
     if (SIGMOID) {
         float high = 0.f;
@@ -289,17 +304,27 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
         for (int i = 0; i < NS; ++i) high = fmaxf(high, x[i]);
         const uint32_t top = __reduce_max_sync(0xffffffffu, order_bits(high));
         m = exact_logit(from_order_bits(top));
-        sum = 0.0;
+        double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
-            if (x[i] > -INFINITY) sum += exp(exact_logit(x[i]) - m);
+        for (int i = 0; i < NS; ++i) {
+            double v = 0.0;
+            if (x[i] > -INFINITY) v = exp(exact_logit(x[i]) - m);
+            if (NS <= 8) e[i < (int)(sizeof(e) / sizeof(double)) ? i : 0] = v;
+            sum += v;
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        inv = 1.0 / sum;
     }
-    auto exact = [&](float v) { return SIGMOID ? exact_sigmoid(v) : (float)(exp(exact_logit(v) - m) / sum); };
+    auto exact = [&](float v) { return SIGMOID ? exact_sigmoid(v) : (float)(exp(exact_logit(v) - m) * inv); };
     if (!sure) {  // the whole warp
 #pragma unroll
-        for (int i = 0; i < NS; ++i) k.c[i] = x[i] > -INFINITY ? __fadd_rn(exact(x[i]), b[i]) : -INFINITY;
+        for (int i = 0; i < NS; ++i) {
+            float s = 0.f;
+            if (!SIGMOID && NS <= 8) s = (float)(e[i < (int)(sizeof(e) / sizeof(double)) ? i : 0] * inv);
+            else if (x[i] > -INFINITY) s = exact(x[i]);
+            k.c[i] = x[i] > -INFINITY ? __fadd_rn(s, b[i]) : -INFINITY;
+        }
         if (a.groups > 1) {
             __syncwarp();
             keep_groups(a, k, by_expert, lane);
@@ -323,7 +348,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
 template <typename T, int NS>
 void launch_route_slots(const RouteArgs& a, bool sigmoid, cudaStream_t stream) {
     const unsigned ctas = (unsigned)(((int64_t)a.rows + kRouteWarps - 1) / kRouteWarps);
-    const int smem = a.groups > 1 && a.experts / a.groups % a.each ? kRouteWarps * a.experts * (int)sizeof(float) : 0;
+    const int smem = a.groups > 1 && !a.span ? kRouteWarps * a.experts * (int)sizeof(float) : 0;
     if (sigmoid) route_kernel<T, NS, true><<<ctas, kRouteThreads, smem, stream>>>(a);
     else route_kernel<T, NS, false><<<ctas, kRouteThreads, smem, stream>>>(a);
 }
@@ -331,6 +356,8 @@ void launch_route_slots(const RouteArgs& a, bool sigmoid, cudaStream_t stream) {
 template <typename T>
 void launch_route_type(RouteArgs a, bool sigmoid, cudaStream_t stream) {
     a.each = (a.experts + 31) / 32;
+    a.size = a.experts / a.groups;
+    a.span = a.size % a.each ? 0 : a.size / a.each;
     int ns = 1;
     while (ns < a.each) ns *= 2;
     a.wide = a.each == ns && a.experts == 32 * ns && ns * sizeof(T) >= 16 &&
@@ -346,7 +373,7 @@ void launch_route_type(RouteArgs a, bool sigmoid, cudaStream_t stream) {
 
 // ---- plan -----------------------------------------------------------------------------------
 
-constexpr int kPlanCluster = 8;
+constexpr int kPlanCluster = 16;  // where the device places it; else the 8 that every one does
 constexpr int kPlanAhead = 4;  // ids a lane has in flight
 
 struct PlanArgs {
@@ -377,16 +404,17 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
     const int64_t run = (((int64_t)a.pairs + ranks * warps - 1) / (ranks * warps) + 31) & ~(int64_t)31;
     const int lo = (int)min((int64_t)a.pairs, run * (rank * warps + warp)), hi = (int)min((int64_t)a.pairs, lo + run);
     auto read = [&](int i) {
-        const int id = i < hi ? __ldg(a.ids + i) : -1;
-        return id >= 0 && id < a.experts ? id : -1;
+        const int id = i < hi ? __ldg(a.ids + i) : a.experts;
+        return id >= 0 && id < a.experts ? id : a.experts;  // nobody's
     };
+    const int bits = 32 - __clz(a.experts);
     for (int i0 = lo; i0 < hi; i0 += 32 * kPlanAhead) {
         int id[kPlanAhead];
 #pragma unroll
         for (int q = 0; q < kPlanAhead; ++q) id[q] = read(i0 + 32 * q + lane);
 #pragma unroll
         for (int q = 0; q < kPlanAhead; ++q)
-            if (id[q] >= 0) atomicAdd(mine + id[q], 1);
+            if (id[q] < a.experts) atomicAdd(mine + id[q], 1);
     }
     __syncthreads();
     for (int e = tid; e < a.experts; e += threads) {
@@ -441,11 +469,17 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
 #pragma unroll
         for (int q = 0; q < kPlanAhead; ++q) {
             const int i = i0 + 32 * q + lane;
-            const unsigned peers = __match_any_sync(0xffffffffu, id[q]);
+            // the lanes with the same id, one ballot for each of its bits
+            unsigned peers = 0xffffffffu;
+            for (int b = 0; b < bits; ++b) {
+                const bool on = id[q] >> b & 1;
+                const unsigned who = __ballot_sync(0xffffffffu, on);
+                peers &= on ? who : ~who;
+            }
             int place = -1;
-            if (id[q] >= 0) place = base[id[q]] + mine[id[q]] + __popc(peers & ((1u << lane) - 1u));
+            if (id[q] < a.experts) place = base[id[q]] + mine[id[q]] + __popc(peers & ((1u << lane) - 1u));
             __syncwarp();
-            if (id[q] >= 0 && lane == __ffs(peers) - 1) mine[id[q]] += __popc(peers);
+            if (id[q] < a.experts && lane == __ffs(peers) - 1) mine[id[q]] += __popc(peers);
             __syncwarp();
             if (i < hi) a.slots[i] = place;
             if (place >= 0) a.order[place] = (int)((unsigned)i / (unsigned)a.k);
@@ -547,11 +581,30 @@ Status launch_route(const void* logits, int dtype, int rows, int experts, int64_
                     int top_k, int sigmoid, int groups, int top_groups, int group_top2, int renormalise, float scale,
                     float* weights, int32_t* ids, cudaStream_t stream) {
     const RouteArgs a{logits, rows, experts, row_stride, bias, top_k, groups, top_groups, group_top2,
-                      renormalise, 0, 0, 0, scale, weights, ids};
+                      renormalise, 0, 0, 0, 0, 0, scale, weights, ids};
     if (dtype == SHIPK_DTYPE_F32) launch_route_type<float>(a, sigmoid, stream);
     else if (dtype == SHIPK_DTYPE_F16) launch_route_type<__half>(a, sigmoid, stream);
     else launch_route_type<__nv_bfloat16>(a, sigmoid, stream);
     return launched();
+}
+
+// Whether a cluster of 16 of these CTAs fits the current device (it need not fit a part of one).
+static bool wide_cluster_fits(cudaLaunchConfig_t config) {
+    static std::mutex mu;
+    static std::map<int, bool> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    std::lock_guard<std::mutex> lock(mu);
+    const auto it = known.find(dev);
+    if (it != known.end()) return it->second;
+    const void* kernel = reinterpret_cast<const void*>(plan_kernel);
+    int n = 0;
+    config.blockDim = dim3(1024);
+    config.dynamicSmemBytes = (size_t)(2 + 32) * kMaxExperts * sizeof(int);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess)
+        cudaGetLastError();  // not fatal: the smaller cluster
+    return known[dev] = n > 0;
 }
 
 Status launch_plan(const int32_t* ids, int rows, int k, int experts, int32_t* order, int32_t* slots, int32_t* offsets,
@@ -559,20 +612,22 @@ Status launch_plan(const int32_t* ids, int rows, int k, int experts, int32_t* or
     const PlanArgs a{ids, rows * k, k, experts, order, slots, offsets};
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(plan_kernel), (2 + 32) * kMaxExperts * (int)sizeof(int));
     if (e != cudaSuccess) return Status{SHIPK_ECUDA, cudaGetErrorString(e)};
-    // a cluster once a CTA's warps would walk for long; a warp for every 128 assignments
-    const int ranks = a.pairs > 8192 ? kPlanCluster : 1;
+    cudaLaunchConfig_t config{};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {kPlanCluster, 1, 1};
+    config.gridDim = dim3(kPlanCluster);
+    config.stream = stream;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    // a cluster once one CTA's warps would walk for long; a warp for every 128 assignments
+    const int ranks = a.pairs <= 2048 ? 1 : wide_cluster_fits(config) ? kPlanCluster : 8;
     const int64_t warps = ((int64_t)a.pairs / ranks + 127) / 128;
     const int threads = 32 * (int)std::min<int64_t>(std::max<int64_t>(warps, 4), 32);
-    cudaLaunchConfig_t config{};
+    attr.val.clusterDim.x = (unsigned)ranks;
     config.gridDim = dim3((unsigned)ranks);
     config.blockDim = dim3((unsigned)threads);
     config.dynamicSmemBytes = (size_t)(2 + threads / 32) * experts * sizeof(int);
-    config.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {(unsigned)ranks, 1, 1};
-    config.attrs = &attr;
-    config.numAttrs = 1;
     e = cudaLaunchKernelEx(&config, plan_kernel, a);
     const Status s = launched();
     return e == cudaSuccess ? s : Status{SHIPK_ECUDA, cudaGetErrorString(e)};
