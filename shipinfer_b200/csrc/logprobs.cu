@@ -825,6 +825,100 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
     }
 }
 
+// Rows of up to 1024 scores: a warp each, every score in a register: score 32 i + lane in slot i, so a
+// slot's 32 bits of the mask are one word. Two passes over the registers, the maximum first; the
+// alternatives one after another.
+template <typename T, int NS, bool MASK>
+__global__ void __launch_bounds__(kWarpCta) logprobs_small_kernel(const __grid_constant__ Args a) {
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * (kWarpCta / 32) + threadIdx.x / 32;
+    if (row >= a.rows) return;
+    const T* logits = static_cast<const T*>(a.logits) + row * a.row_stride;
+    const uint32_t* allowed = MASK ? a.allowed + row * a.allowed_stride : nullptr;
+    float x[NS];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) x[i] = 32 * i + lane < a.vocab ? to_f32(logits[32 * i + lane]) : -INFINITY;
+    // the first given token of this lane, on its way while the row is summed
+    int64_t token = -1;
+    float given = -INFINITY;
+    if (lane < a.n_tokens) {
+        token = a.tokens[row * a.n_tokens + lane];
+        if (token >= 0 && token < a.vocab && (!MASK || (allowed[token >> 5] >> (token & 31)) & 1u)) given = to_f32(logits[token]);
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        if (MASK && 32 * i < a.vocab) x[i] = (__ldg(allowed + i) >> lane) & 1u ? x[i] : -INFINITY;
+        m = fmaxf(m, x[i]);
+    }
+    uint32_t ord = m > -INFINITY ? order_bits(m) : 0u;  // of the lane's largest left
+    uint32_t high = __reduce_max_sync(0xffffffffu, ord);
+    const float top = high ? from_order_bits(high) : 0.f;
+    float s = 0.f, h = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const float y = max_nan((x[i] - top) * a.scale, -150.f), e = exp2_fast(y);
+        s += e;
+        h = __fmaf_rn(e, y, h);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        h += __shfl_xor_sync(0xffffffffu, h, o);
+    }
+    const bool empty = s == 0.f;
+    const float log_s = empty ? 0.f : logf(s);
+    auto logprob = [&](float v) {
+        if (empty || (v == -INFINITY && s == s)) return -INFINITY;
+        return (v - top) * a.inv_t - log_s;  // NaN where S is
+    };
+    if (lane == 0) a.entropy[row] = empty ? 0.f : log_s - 0.693147180559945f * (h / s);
+    for (int j = lane; j < a.n_tokens; j += 32) {
+        if (j >= 32) {
+            token = a.tokens[row * a.n_tokens + j];
+            given = -INFINITY;
+            if (token >= 0 && token < a.vocab && (!MASK || (allowed[token >> 5] >> (token & 31)) & 1u)) given = to_f32(logits[token]);
+        }
+        a.logprobs[row * a.n_tokens + j] = token < 0 ? 0.f : token >= a.vocab ? NAN : logprob(given);
+    }
+    float alternative = 0.f;  // lane j keeps the j-th of each 32
+    int id = -1;
+    for (int j = 0; j < a.top; ++j) {
+        int e = -1;
+        if (high) {
+            // the lowest id with this logit: every lane's lowest slot that has it, then the least of them
+            int slot = 0;
+#pragma unroll
+            for (int i = NS - 1; i >= 0; --i) slot = x[i] >= m ? i : slot;  // m is the lane's largest: never NaN
+            e = __reduce_min_sync(0xffffffffu, ord == high ? 32 * slot + lane : 0x7fffffff);
+            const bool own = ord == high && 32 * slot + lane == e;
+            if (NS > 1) {
+                m = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    x[i] = own && i == slot ? -INFINITY : x[i];
+                    m = fmaxf(m, x[i]);
+                }
+            } else if (own) {
+                m = x[0] = -INFINITY;
+            }
+        }
+        if ((j & 31) == lane) {
+            id = e;
+            alternative = high ? from_order_bits(high) : 0.f;
+        }
+        ord = m > -INFINITY ? order_bits(m) : 0u;
+        high = __reduce_max_sync(0xffffffffu, ord);
+        if ((j & 31) == 31 || j + 1 == a.top) {
+            const int k = (j & ~31) + lane;
+            if (k <= j) {
+                a.top_ids[row * a.top + k] = id;
+                a.top_logprobs[row * a.top + k] = id >= 0 ? logprob(alternative) : -INFINITY;
+            }
+        }
+    }
+}
+
 constexpr int kSms = 148;
 constexpr int kWarpVocab = 4096;  // a warp takes rows of up to this many scores
 constexpr int kWarpTop = 20;      // and this many alternatives of its 32 threads' maxima
@@ -853,8 +947,20 @@ cudaError_t launch(const Args& a, int cluster, cudaStream_t stream) {
     return e != cudaSuccess ? e : last;
 }
 
+template <typename T, int NS, bool MASK>
+cudaError_t launch_small(const Args& a, cudaStream_t stream) {
+    constexpr int rows = kWarpCta / 32;
+    logprobs_small_kernel<T, NS, MASK><<<(unsigned)(((int64_t)a.rows + rows - 1) / rows), kWarpCta, 0, stream>>>(a);
+    return cudaGetLastError();
+}
+
 template <typename T, bool MASK>
 cudaError_t launch(const Args& a, cudaStream_t stream) {
+    if (a.vocab <= 32) return launch_small<T, 1, MASK>(a, stream);
+    if (a.vocab <= 128) return launch_small<T, 4, MASK>(a, stream);
+    if (a.vocab <= 256) return launch_small<T, 8, MASK>(a, stream);
+    if (a.vocab <= 512) return launch_small<T, 16, MASK>(a, stream);
+    if (a.vocab <= 1024) return launch_small<T, 32, MASK>(a, stream);
     if (a.vocab <= kWarpVocab && a.top <= kWarpTop) return launch<T, 32, MASK, false>(a, 1, stream);
     int cluster = 1;
     while (cluster < kMaxCluster && (int64_t)a.rows * cluster <= kSms && a.vocab / cluster > 8192) cluster *= 2;
