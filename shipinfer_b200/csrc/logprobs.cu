@@ -920,8 +920,7 @@ __global__ void __launch_bounds__(kWarpCta) logprobs_small_kernel(const __grid_c
 }
 
 constexpr int kSms = 148;
-constexpr int kWarpVocab = 4096;  // a warp takes rows of up to this many scores
-constexpr int kWarpTop = 20;      // and this many alternatives of its 32 threads' maxima
+constexpr int kWarpTop = 20;  // alternatives that 32 threads' maxima bound
 
 template <typename T, int THREADS, bool MASK, bool CLUSTER>
 cudaError_t launch(const Args& a, int cluster, cudaStream_t stream) {
@@ -961,9 +960,17 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
     if (a.vocab <= 256) return launch_small<T, 8, MASK>(a, stream);
     if (a.vocab <= 512) return launch_small<T, 16, MASK>(a, stream);
     if (a.vocab <= 1024) return launch_small<T, 32, MASK>(a, stream);
-    if (a.vocab <= kWarpVocab && a.top <= kWarpTop) return launch<T, 32, MASK, false>(a, 1, stream);
+    // A warp per row has no barriers and leaves a row's end to the other 31 warps of its SM, but a
+    // row takes it eight times as long: it wins once there are about as many rows as granules in
+    // one. bfloat16, 8 alternatives, warp against CTA in us: 2048 x 8000 15 and 25, 592 x 8000 12 and 9;
+    // 8192 x 32,000 123 and 152, 1024 x 32,000 29 and 25; 16,384 x 1500 40 and 209, 148 x 1500 8.4 and 8.3.
+    const int granules = (int)((int64_t)a.vocab * (int)sizeof(T) / 16);
+    if (a.rows >= granules && a.top <= kWarpTop) return launch<T, 32, MASK, false>(a, 1, stream);
+    // Parts of a row pay where there are CTAs to spare and the pass is long against what a part costs beyond it
+    // (CTA against the best cluster in us: 1 x 128,000 14.4 and 8.6, 64 x 128,000 15.9 and 11.6,
+    // 148 x 128,000 16.9 and 15.7, 64 x 32,000 8.3 and 8.5).
     int cluster = 1;
-    while (cluster < kMaxCluster && (int64_t)a.rows * cluster <= kSms && a.vocab / cluster > 8192) cluster *= 2;
+    while (cluster < kMaxCluster && (int64_t)a.rows * cluster <= kSms && granules / cluster > 4000) cluster *= 2;
     if (cluster == 1) return launch<T, 256, MASK, false>(a, 1, stream);
     return launch<T, 256, MASK, true>(a, cluster, stream);
 }
