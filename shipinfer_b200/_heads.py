@@ -16,6 +16,7 @@ _SAME_DEVICE = nullcontext()
 #: torch's current stream on a device as a handle, without the stream object that
 #: torch.cuda.current_stream() builds around it (2 us of a call whose kernel takes 3)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def element_code(t: Any, name: str) -> int:
@@ -49,39 +50,40 @@ def check_matrix(t: Any, name: str) -> tuple[int, int]:
 
 
 def check_dense(t: Any, name: str, dtype: Any, shape: tuple[int, ...]) -> None:
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValidationError(
             f"{name} must be a contiguous {str(dtype).removeprefix('torch.')} {list(shape)} CUDA tensor; "
             f"got {t.dtype} {list(t.shape)}"
         )
 
 
-def check_device(like: Any, **others: Any) -> Any:
-    """The CUDA device that every tensor of the call is on."""
-    device = like.device
-    for name, t in others.items():
-        if t is not None and t.device != device:
-            raise ValidationError(f"{name} is on {t.device}, another tensor of the call on {device}")
-    if device.type != "cuda":
-        raise ValidationError(f"the tensors of the call must be CUDA tensors; they are on {device}")
-    return device
+def check_device(*tensors: Any) -> int:
+    """The CUDA device that every tensor of the call is on (``None``: not given)."""
+    index = tensors[0].get_device()
+    if index < 0:
+        raise ValidationError(f"the tensors of the call must be CUDA tensors; one is on {tensors[0].device}")
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValidationError(f"a tensor of the call is on {t.device}, another on cuda:{index}")
+    return index
 
 
-def guard(device: Any) -> Any:
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def guard(index: int) -> Any:
+    return _SAME_DEVICE if _get_device() == index else torch.cuda.device(index)
 
 
-def handle_of(device: Any, stream: int | None) -> int:
+def handle_of(index: int, stream: int | None) -> int:
     """The launch's stream: the one given, else torch's current stream on the device."""
     if stream is not None:
         return int(stream)
     if _raw_stream is not None:
-        return _raw_stream(device.index)
-    return torch.cuda.current_stream(device).cuda_stream
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
 
 
-def empty(shape: tuple[int, ...], dtype: Any, device: Any, stream: int | None) -> Any:
+def empty(shape: tuple[int, ...], dtype: Any, index: int, stream: int | None) -> Any:
     """A result of the call, allocated on the stream that writes it."""
+    device = torch.device("cuda", index)
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
     on = torch.cuda.ExternalStream(int(stream), device=device) if stream else torch.cuda.default_stream(device)
@@ -90,4 +92,4 @@ def empty(shape: tuple[int, ...], dtype: Any, device: Any, stream: int | None) -
 
 
 def ptr(t: Any) -> int | None:
-    return t.data_ptr() if t is not None and t.numel() else None
+    return None if t is None else t.data_ptr()  # 0, a null pointer, for an empty tensor

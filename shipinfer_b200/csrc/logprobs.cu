@@ -232,6 +232,9 @@ struct Granule<__half> : Granule16<HalfPair> {};
 __device__ __forceinline__ void copy_async(uint32_t to, const uint4* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+__device__ __forceinline__ void copy_async4(uint32_t to, const uint32_t* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -262,6 +265,13 @@ struct Row {
     }
     __device__ __forceinline__ bool on(int v) const { return !MASK || ((__ldg(allowed + (v >> 5)) >> (v & 31)) & 1u); }
     __device__ __forceinline__ float logit(int v) const { return on(v) ? to_f32(x[v]) : -INFINITY; }
+    // a full granule's bytes with what is not allowed at -inf, by mask words that a warp holds for 32
+    // granules in a row, from word `first` of the mask on
+    __device__ __forceinline__ uint4 cover(const uint4& u, int g, const uint32_t* held, int first) const {
+        if (!MASK) return u;
+        const int v = g * kVec - shift, w = (v >> 5) - first;
+        return Granule<T>::cover(u, __funnelshift_r(held[w], held[w + 1], v & 31));
+    }
     // a full granule's bytes with what is not allowed at -inf
     __device__ __forceinline__ uint4 cover(const uint4& u, int g) const {
         if (!MASK) return u;
@@ -692,7 +702,10 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
     constexpr int kVec = Row<T, MASK>::kVec;
     constexpr int kWarps = THREADS / 32, kGroups = kCta<THREADS> / THREADS;
     constexpr int kStage = kUnroll * THREADS;  // granules
-    extern __shared__ uint4 rings[];           // [kGroups][kStages][kUnroll][THREADS]
+    // of 32 granules in a row: the words that hold their bits, and one that may be read beside them
+    constexpr int kWords = kVec + 2;
+    extern __shared__ uint4 rings[];  // [kGroups][kStages][kUnroll][THREADS]
+    __shared__ uint32_t mask_rings[MASK ? kCta<THREADS> / 32 * kStages * kUnroll * kWords : 1];
     __shared__ Shared<THREADS> shared[kGroups];
     __shared__ uint64_t cluster_keys[CLUSTER ? kMaxCluster * kMaxTop : 1];
     __shared__ Part cluster_parts[CLUSTER ? kMaxCluster : 1];
@@ -714,11 +727,18 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
     int64_t ahead = first;
     const uint4* next = nullptr;
     int left = 0;
+    const uint32_t* mask = nullptr;  // and the row's mask
+    int next_bit = 0;                // with this warp's first granule's bit in it
+    uint32_t* const mask_ring = mask_rings + (MASK ? threadIdx.x / 32 * kStages * kUnroll * kWords : 0);
     auto enter = [&]() {
         const Row<T, MASK> r(a, ahead);
         const Run<T, MASK, THREADS> run(r, part, parts);
         next = r.base + run.from + tid;
         left = run.to - run.from;
+        if (MASK) {
+            mask = r.allowed;
+            next_bit = (run.from + tid - lane) * kVec - r.shift;
+        }
     };
     if (ahead < a.rows) enter();
     auto copy_stage = [&](int stage) {
@@ -734,6 +754,15 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k)
                 if (k * THREADS + tid < left) copy_async(to + k * THREADS * sizeof(uint4), next + k * THREADS);
+        }
+        if (MASK) {  // a lane for each word that the warp's granules of this stage need
+            for (int w = lane; w < kUnroll * (kWords - 1); w += 32) {
+                const int k = w / (kWords - 1), word = ((next_bit + k * THREADS * kVec) >> 5) + w % (kWords - 1);
+                if (k * THREADS + tid - lane < left && word <= (a.vocab - 1) >> 5)
+                    copy_async4((uint32_t)__cvta_generic_to_shared(mask_ring + (stage * kUnroll + k) * kWords + w % (kWords - 1)),
+                                mask + word);
+            }
+            next_bit += kStage * kVec;
         }
         next += kStage;
         left -= kStage;
@@ -758,17 +787,22 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
         float marked = -INFINITY;
         for (int k0 = 0; k0 < stages; ++k0) {
             copies_wait<kStages - 1>();
+            if (MASK) __syncwarp();  // the mask's words are other lanes' copies
             const uint4* held = ring + stage * kStage;
             const int at = run.from + k0 * kStage + tid;
             uint4 u[kUnroll];
+            auto covered = [&](int k) {
+                const int first = ((at - lane + k * THREADS) * kVec - r.shift) >> 5;
+                return r.cover(held[k * THREADS], at + k * THREADS, mask_ring + (stage * kUnroll + k) * kWords, first);
+            };
             if (at - tid + kStage <= run.to) {
 #pragma unroll
-                for (int k = 0; k < kUnroll; ++k) u[k] = r.cover(held[k * THREADS], at + k * THREADS);
+                for (int k = 0; k < kUnroll; ++k) u[k] = covered(k);
             } else {
 #pragma unroll
-                for (int k = 0; k < kUnroll; ++k)
-                    u[k] = at + k * THREADS < run.to ? r.cover(held[k * THREADS], at + k * THREADS) : Granule<T>::empty();
+                for (int k = 0; k < kUnroll; ++k) u[k] = at + k * THREADS < run.to ? covered(k) : Granule<T>::empty();
             }
+            if (MASK) __syncwarp();  // and this stage's are read before the next copies replace them
             marked = fmaxf(marked, sums.take(u, a.scale, a.headroom));
             copy_stage(stage);
             stage = stage + 1 == kStages ? 0 : stage + 1;

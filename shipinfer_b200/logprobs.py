@@ -72,7 +72,7 @@ def token_logprobs_device(
     if tokens is None:
         n, shape = 0, (rows, 0)
     else:
-        shape = tuple(tokens.shape)
+        shape = tokens.shape
         if len(shape) not in (1, 2) or shape[0] != rows:
             raise ValidationError(f"tokens must be [{rows}] or [{rows}, n]; got {list(shape)}")
         n = 1 if len(shape) == 1 else small(shape[1], "tokens per row")
@@ -97,8 +97,7 @@ def token_logprobs_device(
         check_dense(top_logprobs, "top_logprobs", torch.float32, (rows, top))
     if top_ids is not None:
         check_dense(top_ids, "top_ids", torch.int64, (rows, top))
-    dev = check_device(logits, tokens=tokens, allowed=allowed, logprobs=logprobs, entropy=entropy,
-                       top_logprobs=top_logprobs, top_ids=top_ids)
+    dev = check_device(logits, tokens, allowed, logprobs, entropy, top_logprobs, top_ids)
     if logprobs is None:
         logprobs = empty(shape, torch.float32, dev, stream)
     if entropy is None:

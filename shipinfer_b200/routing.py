@@ -79,7 +79,7 @@ def route_experts_device(
         check_dense(weights, "weights", torch.float32, (rows, top_k))
     if ids is not None:
         check_dense(ids, "ids", torch.int32, (rows, top_k))
-    dev = check_device(logits, bias=bias, weights=weights, ids=ids)
+    dev = check_device(logits, bias, weights, ids)
     if weights is None:
         weights = empty((rows, max(top_k, 0)), torch.float32, dev, stream)
     if ids is None:
@@ -130,7 +130,7 @@ def plan_experts_device(
         check_dense(slots, "slots", torch.int32, (rows, k))
     if offsets is not None:
         check_dense(offsets, "offsets", torch.int32, (experts + 1,))
-    dev = check_device(ids, order=order, slots=slots, offsets=offsets)
+    dev = check_device(ids, order, slots, offsets)
     if order is None:
         order = empty((rows * k,), torch.int32, dev, stream)
     if slots is None:
@@ -175,7 +175,7 @@ def combine_experts_device(
     check_dense(weights, "weights", torch.float32, (r, k))
     if out is not None:
         check_dense(out, "out", rows.dtype, (r, width))
-    dev = check_device(slots, weights=weights, rows=rows, out=out)
+    dev = check_device(slots, weights, rows, out)
     if out is None:
         out = empty((r, width), rows.dtype, dev, stream)
     with guard(dev):
