@@ -13,7 +13,7 @@
 // running maximum would at every new one. The threads' sums meet by one rescaling each.
 //
 // The alternatives come out of the same pass. It keeps each thread's largest logit, and a 16-bit
-// mark for each run of granules that the thread read: the largest logit there, rounded down. A
+// mark for each run of granules that the thread read: the upper half of the largest logit there. A
 // bound t that at least `top` of the threads' maxima reach is reached by every alternative, and
 // only runs whose mark reaches it can hold one. These few runs are read again (from L2), what
 // reaches t is collected, and the few dozen collected are ranked.
@@ -369,7 +369,7 @@ struct Running {
     __device__ __forceinline__ float take(const uint4 (&u)[kUnroll], float scale, float headroom) {
         const float top = Granule<T>::largest(u);
         best = fmaxf(best, top);
-        if (!(top <= limit)) {
+        if (__builtin_expect(!(top <= limit), 0)) {
             raise(top, scale, headroom);
             if (limit != limit) {
 #pragma unroll 1
@@ -425,7 +425,7 @@ struct Shared {
     Part parts[THREADS / 32];
     uint32_t rounds[THREADS / 32];     // a warp's contribution to the bound
     uint32_t ord[THREADS];             // order bits of the threads' maxima, 0: none
-    uint16_t marks[kMarks * THREADS];  // upper half of the order bits of a run's largest logit
+    uint16_t marks[kMarks * THREADS];  // upper half of a run's largest logit
     uint16_t runs[kCollect];           // marked runs to read again: mark * THREADS + thread
     int marked, collected;
     uint32_t bound;
@@ -628,8 +628,11 @@ __device__ __forceinline__ void choose(Shared<THREADS>& g, const Row<T, MASK>& r
         }
     };
     if (ord && ord >= t) {
+        // Both cut towards zero, which keeps their order: a run with a logit that reaches t has a mark
+        // that reaches t's upper half.
+        const float least = t ? __uint_as_float(__float_as_uint(from_order_bits(t)) & 0xffff0000u) : -INFINITY;
         for (int m = 0; m < marks; ++m) {
-            if (g.marks[m * THREADS + tid] < t >> 16) continue;
+            if (!(__uint_as_float((uint32_t)g.marks[m * THREADS + tid] << 16) >= least)) continue;
             const int n = atomicAdd(&g.marked, 1);
             if (n < kHold) g.runs[n] = (uint16_t)(m * THREADS + tid);
         }
@@ -741,12 +744,14 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
         }
     };
     if (ahead < a.rows) enter();
-    auto copy_stage = [&](int stage) {
-        while (left <= 0 && ahead < a.rows) {
-            ahead += step;
-            if (ahead < a.rows) enter();
+    auto copy_stage = [&](int slot) {
+        const uint32_t to = ring_at + (uint32_t)(slot * sizeof(uint4));
+        if (left < kStage) {
+            while (left <= 0 && ahead < a.rows) {
+                ahead += step;
+                if (ahead < a.rows) enter();
+            }
         }
-        const uint32_t to = ring_at + (uint32_t)(stage * kStage * sizeof(uint4));
         if (left >= kStage) {
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k) copy_async(to + k * THREADS * sizeof(uint4), next + k * THREADS);
@@ -759,7 +764,7 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
             for (int w = lane; w < kUnroll * (kWords - 1); w += 32) {
                 const int k = w / (kWords - 1), word = ((next_bit + k * THREADS * kVec) >> 5) + w % (kWords - 1);
                 if (k * THREADS + tid - lane < left && word <= (a.vocab - 1) >> 5)
-                    copy_async4((uint32_t)__cvta_generic_to_shared(mask_ring + (stage * kUnroll + k) * kWords + w % (kWords - 1)),
+                    copy_async4((uint32_t)__cvta_generic_to_shared(mask_ring + (slot / THREADS + k) * kWords + w % (kWords - 1)),
                                 mask + word);
             }
             next_bit += kStage * kVec;
@@ -769,8 +774,8 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
         copies_commit();
     };
 #pragma unroll
-    for (int k = 0; k < kStages; ++k) copy_stage(k);
-    int stage = 0;
+    for (int k = 0; k < kStages; ++k) copy_stage(k * kStage);
+    int slot = 0;  // where the next stage to read is in the ring
 
     for (int64_t row = first; row < a.rows; row += step) {
         const Row<T, MASK> r(a, row);
@@ -785,31 +790,31 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
         const int stages = (max(0, run.to - run.from) + kStage - 1) / kStage;
         const int per = stages > Shared<THREADS>::kMarks ? 32 - __clz((stages - 1) / Shared<THREADS>::kMarks) : 0;
         float marked = -INFINITY;
+        const int granules = run.to - run.from;
         for (int k0 = 0; k0 < stages; ++k0) {
             copies_wait<kStages - 1>();
             if (MASK) __syncwarp();  // the mask's words are other lanes' copies
-            const uint4* held = ring + stage * kStage;
-            const int at = run.from + k0 * kStage + tid;
+            const uint4* held = ring + slot;
+            const int done = k0 * kStage;
             uint4 u[kUnroll];
             auto covered = [&](int k) {
-                const int first = ((at - lane + k * THREADS) * kVec - r.shift) >> 5;
-                return r.cover(held[k * THREADS], at + k * THREADS, mask_ring + (stage * kUnroll + k) * kWords, first);
+                const int at = run.from + done + tid + k * THREADS;
+                return r.cover(held[k * THREADS], at, mask_ring + (slot / THREADS + k) * kWords,
+                               ((at - lane) * kVec - r.shift) >> 5);
             };
-            if (at - tid + kStage <= run.to) {
+            if (done + kStage <= granules) {
 #pragma unroll
                 for (int k = 0; k < kUnroll; ++k) u[k] = covered(k);
             } else {
 #pragma unroll
-                for (int k = 0; k < kUnroll; ++k) u[k] = at + k * THREADS < run.to ? covered(k) : Granule<T>::empty();
+                for (int k = 0; k < kUnroll; ++k) u[k] = done + k * THREADS + tid < granules ? covered(k) : Granule<T>::empty();
             }
             if (MASK) __syncwarp();  // and this stage's are read before the next copies replace them
-            marked = fmaxf(marked, sums.take(u, a.scale, a.headroom));
-            copy_stage(stage);
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-            if (((k0 + 1) & ((1 << per) - 1)) == 0 || k0 + 1 == stages) {
-                g.marks[(k0 >> per) * THREADS + tid] = (uint16_t)(order_bits(marked) >> 16);
-                marked = -INFINITY;
-            }
+            const float top = sums.take(u, a.scale, a.headroom);
+            copy_stage(slot);
+            slot = slot == (kStages - 1) * kStage ? 0 : slot + kStage;
+            marked = k0 & ((1 << per) - 1) ? fmaxf(marked, top) : top;
+            g.marks[(k0 >> per) * THREADS + tid] = (uint16_t)(__float_as_uint(marked) >> 16);
         }
         if (run.last(r, tid)) {
             float x[kVec];
