@@ -101,12 +101,7 @@ def test_masks(cuda, dtype, vocab, shared):
     check(cuda, x, tokens, allowed=allowed[0] if shared else allowed, top=min(vocab, 8), temperature=1.6)
 
 
-@pytest.mark.parametrize("vocab", [40, 3001, 60000])
-@pytest.mark.parametrize("dtype", TYPES)
-def test_extreme_rows(cuda, vocab, dtype):
-    """Rows of -inf, of the type's lowest value, of one value, of two far ones; NaN and +inf; a
-    rising and a falling row; signed zeros; all large values in a few places that one thread reads."""
-    torch = cuda
+def extreme_rows(torch, vocab, dtype):
     t = getattr(torch, dtype)
     low = torch.finfo(t).min
     x = torch.zeros((12, vocab), dtype=torch.float32)
@@ -125,10 +120,60 @@ def test_extreme_rows(cuda, vocab, dtype):
     x[10] = -np.inf
     x[10, vocab - 1] = -3.0
     x[11] = torch.arange(vocab) % 2 * 5.0
-    x = x.to(t).cuda()
+    return x.to(t).cuda()
+
+
+@pytest.mark.parametrize("vocab", [40, 3001, 60000])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_extreme_rows(cuda, vocab, dtype):
+    """Rows of -inf, of the type's lowest value, of one value, of two far ones; NaN and +inf; a
+    rising and a falling row; signed zeros; all large values in a few places that one thread reads."""
+    x = extreme_rows(cuda, vocab, dtype)
     tokens = np.tile(np.array([0, vocab - 1, -1, vocab // 2, -7], np.int64), (12, 1))
     check(cuda, x, tokens, top=min(vocab, 33))
     check(cuda, x, tokens, top=min(vocab, 64), temperature=0.01)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_of_middling_length(cuda, dtype):
+    """More rows than a row has 16-byte granules, on and off their boundaries: the extreme rows and
+    ordinary ones, plain and under masks with cleared and single-token rows."""
+    torch = cuda
+    for vocab, rows in ((1100, 420), (3001, 800)):
+        x = scores(torch, rows, vocab, dtype, vocab, pad=3)
+        x[5::7][:12] = extreme_rows(torch, vocab, dtype)[: len(x[5::7][:12])]
+        rng = np.random.default_rng(vocab)
+        tokens = rng.integers(-1, vocab, (rows, 2))
+        check(torch, x, tokens, top=20)
+        check(torch, x.contiguous()[:, 1:], np.minimum(tokens, vocab - 2), top=3, temperature=1.6)
+        allowed = rng.random((rows, vocab)) < 0.5
+        allowed[7], allowed[8] = False, False
+        allowed[8, vocab - 2] = True
+        allowed[9, 40:] = False
+        check(torch, x, tokens, top=8, allowed=allowed)
+        check(torch, x, tokens, top=1, allowed=allowed[3])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_rows_that_follow_one_another(cuda, dtype):
+    """Several long rows for each CTA: a row's copies begin while the one before is ranked."""
+    rows, vocab = 1300, 12001
+    x = scores(cuda, rows, vocab, dtype, 77, pad=2)
+    rng = np.random.default_rng(5)
+    tokens = rng.integers(-1, vocab, (rows, 1))
+    check(cuda, x, tokens, top=24)
+    allowed = rng.random((rows, vocab)) < 0.7
+    allowed[600:610] = False
+    check(cuda, x, tokens, top=7, allowed=allowed)
+
+
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 1e3, 1e6])
+@pytest.mark.parametrize(("rows", "vocab"), [(5, 97), (2, 5003), (700, 1500)])
+def test_far_temperatures(cuda, rows, vocab, temperature):
+    for dtype in TYPES:
+        x = scores(cuda, rows, vocab, dtype, 6)
+        tokens = np.random.default_rng(1).integers(0, vocab, (rows, 2))
+        check(cuda, x, tokens, top=5, temperature=temperature)
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
