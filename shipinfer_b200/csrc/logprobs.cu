@@ -23,6 +23,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cg = cooperative_groups;
 
@@ -36,6 +37,7 @@ constexpr int kUnroll = 4;     // granules (16 bytes) of a thread in a stage
 constexpr int kUnrollLog = 2;
 constexpr int kStages = 2;     // stages a thread has in flight
 static_assert(kUnroll == 1 << kUnrollLog, "");
+constexpr int kMaxRounds = kMaxTop / 8 + 4;  // maxima that a warp of eight offers for the bound
 
 struct Args {
     const void* logits;
@@ -431,6 +433,17 @@ struct Shared {
     uint32_t bound;
 };
 
+// What a CTA that walks over its rows also keeps: the largest maxima of each warp, and, while the
+// next row is read, what it is still to do for the one before.
+struct Walk {
+    static constexpr int kLooks = 256;  // granules that are read again, one for each thread
+    uint4 again[kLooks];
+    int at[kLooks];
+    uint32_t maxima[8 * kMaxRounds];
+    Part sums;
+    int looks;
+};
+
 template <int THREADS>
 __device__ __forceinline__ void group_sync() {
     if (THREADS == 32) __syncwarp();
@@ -594,6 +607,67 @@ __device__ __noinline__ bool collect_ties(Shared<THREADS>& g, Row<T, MASK> r, Ru
     return true;
 }
 
+// What is collected, best first, into g.chosen; by the ways for more than was held where it was more.
+template <typename T, bool MASK, int THREADS>
+__device__ __forceinline__ void rank(Shared<THREADS>& g, const Row<T, MASK>& r, const Run<T, MASK, THREADS>& run,
+                                     int wanted, int tid, uint32_t t) {
+    constexpr int kHold = Shared<THREADS>::kCollect;
+    bool held = g.collected <= kHold && g.marked <= kHold;
+    if (!held) held = collect_ties<T, MASK, THREADS>(g, r, run, wanted, tid, t);
+    if (held) {
+        const int n = g.collected;
+        for (int i = tid; i < n; i += THREADS) {
+            const uint64_t k = g.keys[i];
+            int better = 0;
+            for (int j = 0; j < n; ++j) better += g.keys[j] > k;
+            if (better < wanted) g.chosen[better] = k;
+        }
+    } else {
+        choose_slowly<T, MASK, THREADS>(g, r, run, wanted, tid);
+    }
+    group_sync<THREADS>();
+}
+
+// Collect what reaches the bound among a granule's scores.
+template <int VEC, int THREADS>
+__device__ __forceinline__ void collect(Shared<THREADS>& g, const float (&x)[VEC], int at, int shift, uint32_t t) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        if (!(x[i] > -INFINITY && order_bits(x[i]) >= t)) continue;
+        const int n = atomicAdd(&g.collected, 1);
+        if (n < Shared<THREADS>::kCollect) g.keys[n] = choice_key(x[i], at * VEC - shift + i);
+    }
+}
+
+// This thread's runs whose marks reach the bound, if its maximum does, and its ends of the row.
+template <typename T, bool MASK, int THREADS>
+__device__ __forceinline__ void mark_runs(Shared<THREADS>& g, const Row<T, MASK>& r, const Run<T, MASK, THREADS>& run,
+                                          int tid, uint32_t ord, uint32_t t, int marks) {
+    constexpr int kVec = Row<T, MASK>::kVec;
+    if (!(ord && ord >= t)) return;
+    // Both cut towards zero, which keeps their order: a run with a logit that reaches t has a mark
+    // that reaches t's upper half.
+    const float least = t ? __uint_as_float(__float_as_uint(from_order_bits(t)) & 0xffff0000u) : -INFINITY;
+    for (int m = 0; m < marks; ++m) {
+        if (!(__uint_as_float((uint32_t)g.marks[m * THREADS + tid] << 16) >= least)) continue;
+        const int n = atomicAdd(&g.marked, 1);
+        if (n < Shared<THREADS>::kCollect) g.runs[n] = (uint16_t)(m * THREADS + tid);
+    }
+    if (run.first(r, tid) || run.last(r, tid)) {
+        float x[kVec];
+        const int at = tid == 0 ? 0 : run.g1 - 1;
+        r.read(at, x);
+        collect<kVec, THREADS>(g, x, at, r.shift, t);
+    }
+}
+
+// The granule of the q-th look at the marked runs of 2^shift granules each; run.to: none.
+template <typename T, bool MASK, int THREADS>
+__device__ __forceinline__ int look_at(const Shared<THREADS>& g, const Run<T, MASK, THREADS>& run, int q, int shift) {
+    const int of = g.runs[q >> shift], k = q & ((1 << shift) - 1);
+    return min(run.to, run.from + of % THREADS + (((of / THREADS) << shift) + k) * THREADS);
+}
+
 // The alternatives among a run's granules into g.chosen, best first, 0 past the last; called by the
 // whole group with each thread's largest logit, which is in g.ord, and, for more than one warp,
 // with the warps' parts of the bound in g.rounds. Each of a thread's `marks` marks stands for
@@ -603,7 +677,6 @@ __device__ __forceinline__ void choose(Shared<THREADS>& g, const Row<T, MASK>& r
                                        int wanted, int tid, uint32_t ord, int marks, int shift) {
     constexpr int kVec = Row<T, MASK>::kVec;
     constexpr int kWarps = THREADS / 32;
-    constexpr int kHold = Shared<THREADS>::kCollect;
     uint32_t t;
     if (kWarps == 1) {
         t = find_bound<THREADS>(g, wanted, tid);
@@ -619,55 +692,18 @@ __device__ __forceinline__ void choose(Shared<THREADS>& g, const Row<T, MASK>& r
             t = g.bound;
         }
     }
-    auto look = [&](const float (&x)[kVec], int at) {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            if (!(x[i] > -INFINITY && order_bits(x[i]) >= t)) continue;
-            const int n = atomicAdd(&g.collected, 1);
-            if (n < kHold) g.keys[n] = choice_key(x[i], at * kVec - r.shift + i);
-        }
-    };
-    if (ord && ord >= t) {
-        // Both cut towards zero, which keeps their order: a run with a logit that reaches t has a mark
-        // that reaches t's upper half.
-        const float least = t ? __uint_as_float(__float_as_uint(from_order_bits(t)) & 0xffff0000u) : -INFINITY;
-        for (int m = 0; m < marks; ++m) {
-            if (!(__uint_as_float((uint32_t)g.marks[m * THREADS + tid] << 16) >= least)) continue;
-            const int n = atomicAdd(&g.marked, 1);
-            if (n < kHold) g.runs[n] = (uint16_t)(m * THREADS + tid);
-        }
-        if (run.first(r, tid) || run.last(r, tid)) {
-            float x[kVec];
-            const int at = tid == 0 ? 0 : run.g1 - 1;
-            r.read(at, x);
-            look(x, at);
-        }
-    }
+    mark_runs<T, MASK, THREADS>(g, r, run, tid, ord, t, marks);
     group_sync<THREADS>();
-    const int looks = min(g.marked, kHold) << shift;
+    const int looks = min(g.marked, Shared<THREADS>::kCollect) << shift;
     for (int q = tid; q < looks; q += THREADS) {
-        const int of = g.runs[q >> shift], k = q & ((1 << shift) - 1);
-        const int at = run.from + of % THREADS + (((of / THREADS) << shift) + k) * THREADS;
+        const int at = look_at<T, MASK, THREADS>(g, run, q, shift);
         if (at >= run.to) continue;
         float x[kVec];
         Granule<T>::unpack(r.cover(__ldg(r.base + at), at), x);
-        look(x, at);
+        collect<kVec, THREADS>(g, x, at, r.shift, t);
     }
     group_sync<THREADS>();
-    bool held = g.collected <= kHold && g.marked <= kHold;
-    if (!held) held = collect_ties<T, MASK, THREADS>(g, r, run, wanted, tid, t);
-    if (held) {
-        const int n = g.collected;
-        for (int i = tid; i < n; i += THREADS) {
-            const uint64_t k = g.keys[i];
-            int better = 0;
-            for (int j = 0; j < n; ++j) better += g.keys[j] > k;
-            if (better < wanted) g.chosen[better] = k;
-        }
-    } else {
-        choose_slowly<T, MASK, THREADS>(g, r, run, wanted, tid);
-    }
-    group_sync<THREADS>();
+    rank<T, MASK, THREADS>(g, r, run, wanted, tid, t);
 }
 
 // The row's results from its sums and its alternatives' keys.
@@ -692,8 +728,31 @@ __device__ __forceinline__ void write_row(const Args& a, const Row<T, MASK>& r, 
     }
 }
 
+// What a walking CTA does for a row while it reads the next one. The granules that it asked for when the
+// row ended have come: collect what reaches the bound. Each thread looks at its own copies only.
+template <typename T, bool MASK, int THREADS>
+__device__ __noinline__ void collect_again(const Args& a, Shared<THREADS>& g, const Walk& w, int row, int tid) {
+    constexpr int kVec = Row<T, MASK>::kVec;
+    if (tid >= w.looks || w.at[tid] < 0) return;
+    const Row<T, MASK> r(a, row);
+    float x[kVec];
+    Granule<T>::unpack(r.cover(w.again[tid], w.at[tid]), x);
+    collect<kVec, THREADS>(g, x, w.at[tid], r.shift, g.bound);
+}
+// And then rank it and write the row's results.
+template <typename T, bool MASK, int THREADS>
+__device__ __noinline__ void finish(const Args& a, Shared<THREADS>& g, const Walk& w, int row, int tid) {
+    const Row<T, MASK> r(a, row);
+    const Run<T, MASK, THREADS> run(r, 0, 1);
+    group_sync<THREADS>();
+    rank<T, MASK, THREADS>(g, r, run, a.top, tid, g.bound);
+    write_row<T, MASK, THREADS>(a, r, row, w.sums, g.chosen, tid);
+}
+
 // A group of THREADS threads per row: a warp, a CTA, or (CLUSTER) a CTA for each part of a row.
-// Groups walk over the rows. Each thread copies its granules into places of its own in shared
+// Groups walk over the rows. A walking CTA does not wait for the granules that it reads again (they
+// take 4 us from a busy memory, an eighth of a row of 128,256 bfloat16 scores): it asks for them when the
+// row ends, looks at them after the next row's second stage and ranks them after its third. Each thread copies its granules into places of its own in shared
 // memory, kStages stages of kUnroll ahead of where it reads, past the end of a row into the next
 // one: what a row needs beyond its pass runs while the next row arrives. No thread reads what
 // another copied, so the copies need no barrier.
@@ -709,7 +768,10 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
     constexpr int kWords = kVec + 2;
     extern __shared__ uint4 rings[];  // [kGroups][kStages][kUnroll][THREADS]
     __shared__ uint32_t mask_rings[MASK ? kCta<THREADS> / 32 * kStages * kUnroll * kWords : 1];
+    constexpr bool kWalks = kGroups == 1 && !CLUSTER;
     __shared__ Shared<THREADS> shared[kGroups];
+    __shared__ std::conditional_t<kWalks, Walk, int> walk;
+    int owed = -1;  // the row that is still to be ranked and written
     __shared__ uint64_t cluster_keys[CLUSTER ? kMaxCluster * kMaxTop : 1];
     __shared__ Part cluster_parts[CLUSTER ? kMaxCluster : 1];
     const int group = threadIdx.x / THREADS, tid = threadIdx.x % THREADS, lane = tid & 31;
@@ -815,6 +877,15 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
             slot = slot == (kStages - 1) * kStage ? 0 : slot + kStage;
             marked = k0 & ((1 << per) - 1) ? fmaxf(marked, top) : top;
             g.marks[(k0 >> per) * THREADS + tid] = (uint16_t)(__float_as_uint(marked) >> 16);
+            if constexpr (kWalks) {
+                if (__builtin_expect(owed >= 0, 0)) {
+                    if (k0 == 1) collect_again<T, MASK, THREADS>(a, g, walk, owed, tid);
+                    if (k0 == 2) {
+                        finish<T, MASK, THREADS>(a, g, walk, owed, tid);
+                        owed = -1;
+                    }
+                }
+            }
         }
         if (run.last(r, tid)) {
             float x[kVec];
@@ -823,6 +894,82 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
         }
         Part p = join<32>(sums.part(a.scale), a.scale);
         const uint32_t ord = sums.best > -INFINITY ? order_bits(sums.best) : 0u;
+        const int marks = (stages + (1 << per) - 1) >> per, shift = per + kUnrollLog;
+        if constexpr (kWalks) {
+            if (owed >= 0) {  // this row was a short one
+                copies_wait<0>();
+                if (stages < 2) collect_again<T, MASK, THREADS>(a, g, walk, owed, tid);
+                finish<T, MASK, THREADS>(a, g, walk, owed, tid);
+                owed = -1;
+            }
+            // Each warp offers its largest maxima; the top-th largest of these is the bound: as good
+            // as that of all the maxima unless a warp has more of the best than it offers.
+            const int rounds = (a.top + kWarps - 1) / kWarps + 4;
+            if (lane == 0) g.parts[tid / 32] = p;
+            if (a.top > 0) {
+                g.ord[tid] = ord;
+                if (tid == 0) g.marked = g.collected = 0;
+                uint32_t left = ord;
+                for (int i = 0; i < rounds; ++i) {
+                    const uint32_t high = __reduce_max_sync(0xffffffffu, left);
+                    if (lane == __ffs(__ballot_sync(0xffffffffu, left == high)) - 1) left = 0;
+                    if (lane == 0) walk.maxima[tid / 32 * rounds + i] = high;
+                }
+            }
+            __syncthreads();
+            p = join<kWarps>(g.parts[lane % kWarps], a.scale);
+            if (a.top > 0) {
+                for (int j = tid; j < a.top; j += THREADS) g.chosen[j] = 0;
+                const int offered = kWarps * rounds;
+                if (tid < offered) {
+                    const uint32_t v = walk.maxima[tid];
+                    int before = 0;
+                    for (int j = 0; j < offered; ++j) before += walk.maxima[j] > v || (walk.maxima[j] == v && j < tid);
+                    if (before == a.top - 1) g.bound = v;
+                }
+                __syncthreads();
+                uint32_t t = g.bound;
+                if (!t) {  // warps with few logits, or none: uniform over the CTA
+                    __syncthreads();
+                    if (tid < 32) {
+                        t = find_bound<THREADS>(g, a.top, tid);
+                        if (tid == 0) g.bound = t;
+                    }
+                    __syncthreads();
+                    t = g.bound;
+                }
+                mark_runs<T, MASK, THREADS>(g, r, run, tid, ord, t, marks);
+                __syncthreads();
+                const int looks = min(g.marked, Shared<THREADS>::kCollect) << shift;
+                if (looks <= Walk::kLooks && row + step < a.rows) {  // another row follows
+                    if (tid < looks) {
+                        const int at = look_at<T, MASK, THREADS>(g, run, tid, shift);
+                        walk.at[tid] = at < run.to ? at : -1;
+                        if (at < run.to) copy_async((uint32_t)__cvta_generic_to_shared(walk.again + tid), r.base + at);
+                    }
+                    copies_commit();
+                    if (tid == 0) {
+                        walk.sums = p;
+                        walk.looks = looks;
+                    }
+                    owed = (int)row;
+                    __syncthreads();
+                    continue;
+                }
+                for (int q = tid; q < looks; q += THREADS) {
+                    const int at = look_at<T, MASK, THREADS>(g, run, q, shift);
+                    if (at >= run.to) continue;
+                    float x[Row<T, MASK>::kVec];
+                    Granule<T>::unpack(r.cover(__ldg(r.base + at), at), x);
+                    collect<Row<T, MASK>::kVec, THREADS>(g, x, at, r.shift, t);
+                }
+                __syncthreads();
+                rank<T, MASK, THREADS>(g, r, run, a.top, tid, t);
+            }
+            write_row<T, MASK, THREADS>(a, r, row, p, g.chosen, tid);
+            __syncthreads();  // the next row's threads write where this row's read
+            continue;
+        }
         if (kWarps > 1 && lane == 0) g.parts[tid / 32] = p;
         if (a.top > 0) {
             g.ord[tid] = ord;
@@ -835,8 +982,7 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
         }
         group_sync<THREADS>();
         if (kWarps > 1) p = join<kWarps>(g.parts[lane % kWarps], a.scale);
-        if (a.top > 0)
-            choose<T, MASK, THREADS>(g, r, run, a.top, tid, ord, (stages + (1 << per) - 1) >> per, per + kUnrollLog);
+        if (a.top > 0) choose<T, MASK, THREADS>(g, r, run, a.top, tid, ord, marks, shift);
         if (CLUSTER) {  // its parts meet in its first CTA
             cg::cluster_group cluster = cg::this_cluster();
             cluster.barrier_wait();
