@@ -267,13 +267,6 @@ struct Row {
     }
     __device__ __forceinline__ bool on(int v) const { return !MASK || ((__ldg(allowed + (v >> 5)) >> (v & 31)) & 1u); }
     __device__ __forceinline__ float logit(int v) const { return on(v) ? to_f32(x[v]) : -INFINITY; }
-    // a full granule's bytes with what is not allowed at -inf, by mask words that a warp holds for 32
-    // granules in a row, from word `first` of the mask on
-    __device__ __forceinline__ uint4 cover(const uint4& u, int g, const uint32_t* held, int first) const {
-        if (!MASK) return u;
-        const int v = g * kVec - shift, w = (v >> 5) - first;
-        return Granule<T>::cover(u, __funnelshift_r(held[w], held[w + 1], v & 31));
-    }
     // a full granule's bytes with what is not allowed at -inf
     __device__ __forceinline__ uint4 cover(const uint4& u, int g) const {
         if (!MASK) return u;
@@ -766,6 +759,7 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
     constexpr int kStage = kUnroll * THREADS;  // granules
     // of 32 granules in a row: the words that hold their bits, and one that may be read beside them
     constexpr int kWords = kVec + 2;
+    static_assert(THREADS * kVec % 32 == 0, "the granules of a thread are whole words apart");
     extern __shared__ uint4 rings[];  // [kGroups][kStages][kUnroll][THREADS]
     __shared__ uint32_t mask_rings[MASK ? kCta<THREADS> / 32 * kStages * kUnroll * kWords : 1];
     constexpr bool kWalks = kGroups == 1 && !CLUSTER;
@@ -853,6 +847,9 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
         const int per = stages > Shared<THREADS>::kMarks ? 32 - __clz((stages - 1) / Shared<THREADS>::kMarks) : 0;
         float marked = -INFINITY;
         const int granules = run.to - run.from;
+        // where this thread's bits are among its warp's words: a stage is whole words, so always there
+        const int warp_bit = ((run.from + tid - lane) * kVec - r.shift) & 31, my_bit = (warp_bit + lane * kVec) & 31;
+        const uint32_t* const my_mask = mask_ring + (warp_bit + lane * kVec) / 32;
         for (int k0 = 0; k0 < stages; ++k0) {
             copies_wait<kStages - 1>();
             if (MASK) __syncwarp();  // the mask's words are other lanes' copies
@@ -860,9 +857,9 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
             const int done = k0 * kStage;
             uint4 u[kUnroll];
             auto covered = [&](int k) {
-                const int at = run.from + done + tid + k * THREADS;
-                return r.cover(held[k * THREADS], at, mask_ring + (slot / THREADS + k) * kWords,
-                               ((at - lane) * kVec - r.shift) >> 5);
+                if (!MASK) return held[k * THREADS];
+                const uint32_t* w = my_mask + (slot / THREADS + k) * kWords;
+                return Granule<T>::cover(held[k * THREADS], __funnelshift_r(w[0], w[1], my_bit));
             };
             if (done + kStage <= granules) {
 #pragma unroll
