@@ -117,6 +117,16 @@ __device__ __forceinline__ Part join(Part p, float scale) {
 
 // ---- 16 bytes of scores: one granule ----------------------------------------------------------
 
+// Bits 0 to 3 as the signs of a word's bytes, which a byte permutation spreads over a score.
+__device__ __forceinline__ uint32_t byte_signs(uint32_t bits) { return ((bits & 15u) * 0x10204080u) & 0x80808080u; }
+template <uint32_t SELECTOR>  // a nibble above 7: the sign of that byte, eight times
+__device__ __forceinline__ uint32_t spread(uint32_t signs) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(signs), "n"(SELECTOR));
+    return r;
+}
+__device__ __forceinline__ uint32_t pick(uint32_t on, uint32_t off, uint32_t mask) { return (on & mask) | (off & ~mask); }
+
 template <typename T>
 struct Granule;
 
@@ -149,8 +159,9 @@ struct Granule<float> {
     // whether scaled() may be used with a reference: x scale does not overflow above, -inf is no trouble
     static __device__ __forceinline__ bool plain(float, float) { return true; }
     static __device__ __forceinline__ uint4 cover(const uint4& u, uint32_t bits) {
-        const uint32_t none = 0xff800000u;
-        return make_uint4(bits & 1u ? u.x : none, bits & 2u ? u.y : none, bits & 4u ? u.z : none, bits & 8u ? u.w : none);
+        const uint32_t signs = byte_signs(bits), none = 0xff800000u;
+        return make_uint4(pick(u.x, none, spread<0x8888>(signs)), pick(u.y, none, spread<0x9999>(signs)),
+                          pick(u.z, none, spread<0xaaaa>(signs)), pick(u.w, none, spread<0xbbbb>(signs)));
     }
 };
 
@@ -185,13 +196,10 @@ struct Granule16 {
     // with this reference, a score at the clamp or below has no probability
     static __device__ __forceinline__ bool plain(float ref, float scale) { return (T::kLow - ref) * scale < -150.f; }
     static __device__ __forceinline__ uint4 cover(const uint4& u, uint32_t bits) {
-        uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t on = (bits >> (2 * i) & 1u ? 0xffffu : 0u) | (bits >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
-            w[i] = (w[i] & on) | (T::kNone & ~on);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        const uint32_t low = byte_signs(bits), high = byte_signs(bits >> 4);
+        return make_uint4(pick(u.x, T::kNone, spread<0x9988>(low)), pick(u.y, T::kNone, spread<0xbbaa>(low)),
+                          pick(u.z, T::kNone, spread<0x9988>(high)),
+                          pick(u.w, T::kNone, spread<0xbbaa>(high)));
     }
 };
 struct Bf16Pair {
@@ -787,8 +795,17 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
     const uint4* next = nullptr;
     int left = 0;
     const uint32_t* mask = nullptr;  // and the row's mask
-    int next_bit = 0;                // with this warp's first granule's bit in it
+    int next_word = 0;               // with the word of this warp's first granule in it
+    const int last_word = (a.vocab - 1) >> 5;
     uint32_t* const mask_ring = mask_rings + (MASK ? threadIdx.x / 32 * kStages * kUnroll * kWords : 0);
+    const uint32_t mask_at = (uint32_t)__cvta_generic_to_shared(mask_ring);
+    // the words that a lane copies: how far from the stage's first, and from its place in the ring in bytes
+    constexpr int kNeeded = kUnroll * (kWords - 1);
+    auto word_of = [](int w) {
+        const int k = w / (kWords - 1), i = w % (kWords - 1);
+        return int2{k * (THREADS * kVec / 32) + i, (k * kWords + i) * (int)sizeof(uint32_t)};
+    };
+    const int2 words = word_of(lane), more = word_of(lane + 32);
     auto enter = [&]() {
         const Row<T, MASK> r(a, ahead);
         const Run<T, MASK, THREADS> run(r, part, parts);
@@ -796,7 +813,7 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
         left = run.to - run.from;
         if (MASK) {
             mask = r.allowed;
-            next_bit = (run.from + tid - lane) * kVec - r.shift;
+            next_word = ((run.from + tid - lane) * kVec - r.shift) >> 5;
         }
     };
     if (ahead < a.rows) enter();
@@ -816,14 +833,12 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
             for (int k = 0; k < kUnroll; ++k)
                 if (k * THREADS + tid < left) copy_async(to + k * THREADS * sizeof(uint4), next + k * THREADS);
         }
-        if (MASK) {  // a lane for each word that the warp's granules of this stage need
-            for (int w = lane; w < kUnroll * (kWords - 1); w += 32) {
-                const int k = w / (kWords - 1), word = ((next_bit + k * THREADS * kVec) >> 5) + w % (kWords - 1);
-                if (k * THREADS + tid - lane < left && word <= (a.vocab - 1) >> 5)
-                    copy_async4((uint32_t)__cvta_generic_to_shared(mask_ring + (slot / THREADS + k) * kWords + w % (kWords - 1)),
-                                mask + word);
-            }
-            next_bit += kStage * kVec;
+        if (MASK && left > 0) {  // a lane for each word that the warp's granules of this stage need
+            const uint32_t at = mask_at + (uint32_t)(slot / THREADS * kWords * sizeof(uint32_t));
+            if (lane < kNeeded && next_word + words.x <= last_word) copy_async4(at + words.y, mask + next_word + words.x);
+            if (kNeeded > 32 && lane + 32 < kNeeded && next_word + more.x <= last_word)
+                copy_async4(at + more.y, mask + next_word + more.x);
+            next_word += kStage * kVec / 32;
         }
         next += kStage;
         left -= kStage;
