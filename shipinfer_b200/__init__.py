@@ -7,6 +7,10 @@ crop-resize, and device NMS — as hand-written CUDA behind the C ABI in ``inclu
   ``letterbox_to_device``, ``crop_batch``, ``nms``) plus the device-resident batched API.
 * :class:`ThreadLocalImageOps` — one ``NativeImageOps`` per worker thread, threads spread
   over the GPUs in rotation (the reference's multi-GPU preprocessing wrapper).
+* :mod:`shipinfer_b200.decode`, :mod:`shipinfer_b200.masks` — what detectors and segmenters answer,
+  decoded on the device.
+* :mod:`shipinfer_b200.logprobs`, :mod:`shipinfer_b200.routing` — token log-probabilities of a
+  reader's scores; a gate's scores turned into each embedder's batch of crops and back.
 * :mod:`shipinfer_b200.shipvision_C` — the ``shipvision._C`` surface the reference's loader
   probes, for a drop-in under ``execution.provider=native``.
 

@@ -751,12 +751,21 @@ __device__ __noinline__ void finish(const Args& a, Shared<THREADS>& g, const Wal
 }
 
 // A group of THREADS threads per row: a warp, a CTA, or (CLUSTER) a CTA for each part of a row.
-// Groups walk over the rows. A walking CTA does not wait for the granules that it reads again (they
-// take 4 us from a busy memory, an eighth of a row of 128,256 bfloat16 scores): it asks for them when the
-// row ends, looks at them after the next row's second stage and ranks them after its third. Each thread copies its granules into places of its own in shared
+// Groups walk over the rows. Each thread copies its granules into places of its own in shared
 // memory, kStages stages of kUnroll ahead of where it reads, past the end of a row into the next
-// one: what a row needs beyond its pass runs while the next row arrives. No thread reads what
-// another copied, so the copies need no barrier.
+// one. No thread reads what another copied (but for the mask's words, which a warp shares), so the
+// copies need no barrier. A walking CTA does not wait for the granules that it reads again (they
+// take 4 us from a busy memory, an eighth of a row of 128,256 bfloat16 scores): it asks for them
+// when the row ends, looks at them after the next row's second stage and ranks them after its third.
+//
+// Bound by issue slots and the exponential unit, with the memory close behind: 231 instructions for
+// a thread's stage of 32 bfloat16 scores, 32 of them exponentials, of which an SM starts 16 a clock.
+// 4096 rows of 128,256 bfloat16 scores take 176 us without alternatives and 206 with 20 of them,
+// 2048 rows of float32 170; the scores alone take 161 at the memory's 6.55 TB/s. Dropped, each with
+// 20 alternatives against the kernel of its time: loads into registers, a bound's holders read again
+// whole (276 us); stages half as long (241 against 218), three CTAs of three stages (221), CTAs of 128
+// threads (233), two warps of a CTA that finish what eight read (212 against 214, slower for few
+// rows), a share of the exponentials by multiply-adds (213 to 232 against 213).
 template <int THREADS>
 constexpr int kCta = THREADS == 32 ? kWarpCta : THREADS;
 
@@ -1022,7 +1031,8 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
     }
 }
 
-// Rows of up to 1024 scores: a warp each, every score in a register: score 32 i + lane in slot i, so a
+// Rows of up to 1024 scores: a warp each, bound by the latency of its few steps (4096 rows of 97 float32
+// scores, 3 alternatives, in 4.2 us; the kernel above took 10.5). Every score is in a register: score 32 i + lane in slot i, so a
 // slot's 32 bits of the mask are one word. Two passes over the registers, the maximum first; the
 // alternatives one after another.
 template <typename T, int NS, bool MASK>

@@ -222,7 +222,9 @@ __device__ __forceinline__ bool take_best(const RouteArgs& a, Choices<NS>& k, co
 // (2 units in the last place for the exponential, 2 for the quotient, the sum's rounding: 2^-20.6 of
 // the score) and where all the choices that decide are further apart than two such errors they
 // stand as they would in 64 bits; only else are all of the row's scores computed in 64. The weights
-// always come from the exact scores of the chosen.
+// always come from the exact scores of the chosen. Bound by issue slots (77% busy): 16,384 rows of 256
+// experts in 8 groups, 1160 instructions a row, take 25 us where the logits alone are 2.6; 64 bits
+// for every score and choices in shared memory took 55.
 template <typename T, int NS, bool SIGMOID>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ RouteArgs a) {
     extern __shared__ float route_smem[];
@@ -387,7 +389,11 @@ struct PlanArgs {
 // One CTA, or one cluster of them. Each warp owns a run of assignments and a row of counters: it
 // counts its run's experts, the counters become the places before which this warp's assignments
 // of each expert go (after those of earlier warps, earlier CTAs and lower experts), and it walks its
-// run again in order, so that the sort is stable and no atomic decides a place.
+// run again in order, so that the sort is stable and no atomic decides a place. Bound by what an SM
+// issues and scatters, so by how many SMs a cluster has: 131,072 assignments of 256 experts take 273
+// us on one CTA (with a 64-bit division for each), 21 on a cluster of 8 and 14 on one of 16, the most there is; two
+// launches with the counts in memory between them could use them all, for a workspace and a second
+// launch. Equal ids by one ballot a bit: __match_any_sync took 25 us on the cluster of 8.
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ PlanArgs a) {
     extern __shared__ int plan_smem[];
     __shared__ int scan[32];
