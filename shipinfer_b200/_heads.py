@@ -55,6 +55,8 @@ def check_dense(t: Any, name: str, dtype: Any, shape: tuple[int, ...]) -> None:
             f"{name} must be a contiguous {str(dtype).removeprefix('torch.')} {list(shape)} CUDA tensor; "
             f"got {t.dtype} {list(t.shape)}"
         )
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValidationError(f"{name} asks for a gradient; this call computes none (use no_grad or detach)")
 
 
 def check_device(*tensors: Any) -> int:

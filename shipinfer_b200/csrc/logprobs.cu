@@ -130,7 +130,7 @@ __device__ __forceinline__ uint32_t pick(uint32_t on, uint32_t off, uint32_t mas
 template <typename T>
 struct Granule;
 
-// 32-bit scores. `low` stands in for what has no probability: its 2^y is 0 and y 2^y no NaN.
+// 32-bit scores. What has no probability has its y clamped: 2^y is 0 then, and y 2^y no NaN.
 template <>
 struct Granule<float> {
     static constexpr int kVec = 4;
@@ -320,11 +320,11 @@ struct Run {
 
 // What a thread has of a row while it reads its granules: the sums relative to `ref`, in pairs, and
 // its largest logit. Two ways to add scores. The plain one takes y = x scale + offset in one
-// rounding, with offset = -ref scale rounded: the sums are then relative to the logit whose y is exactly
-// 0, `slip` (in y) away from ref, which part() puts right. The careful one takes (x - ref) scale
-// and clamps each y: for the first scores, where there is no reference yet, for references so
-// large that ref scale says nothing about x scale, and, in 16 bits, for references so low that
-// a score of -inf clamped to a finite one would count.
+// rounding, with offset = -ref scale rounded: the sums are then relative to the logit whose y is
+// exactly 0, `slip` (in y) away from ref, which part() puts right. The careful one takes
+// (x - ref) scale and clamps each y: where there is no reference yet, for references so large that
+// ref scale says nothing about x scale, and, in 16 bits, for references so low that a score of -inf
+// clamped to a finite one would count.
 template <typename T>
 struct Running {
     static constexpr int kVec = Granule<T>::kVec;
@@ -549,8 +549,8 @@ __device__ __noinline__ void choose_slowly(Shared<THREADS>& g, Row<T, MASK> r, R
 }
 
 // For rows where many logits equal the bound t (rows of one value, zeros): what is above t as ever,
-// and the first that equal it, found in the row's order until there are enough. False if more is above
-// t than the group can hold.
+// and the first that equal it, found in the row's order until there are enough. False if more is
+// above t than the group can hold.
 template <typename T, bool MASK, int THREADS>
 __device__ __noinline__ bool collect_ties(Shared<THREADS>& g, Row<T, MASK> r, Run<T, MASK, THREADS> run,
                                           int wanted, int tid, uint32_t t) {
@@ -729,8 +729,8 @@ __device__ __forceinline__ void write_row(const Args& a, const Row<T, MASK>& r, 
     }
 }
 
-// What a walking CTA does for a row while it reads the next one. The granules that it asked for when the
-// row ended have come: collect what reaches the bound. Each thread looks at its own copies only.
+// What a walking CTA does for a row while it reads the next one. The granules that it asked for when
+// the row ended have come: collect what reaches the bound. Each thread looks at its own copies only.
 template <typename T, bool MASK, int THREADS>
 __device__ __noinline__ void collect_again(const Args& a, Shared<THREADS>& g, const Walk& w, int row, int tid) {
     constexpr int kVec = Row<T, MASK>::kVec;
@@ -1167,15 +1167,16 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
     if (a.vocab <= 256) return launch_small<T, 8, MASK>(a, stream);
     if (a.vocab <= 512) return launch_small<T, 16, MASK>(a, stream);
     if (a.vocab <= 1024) return launch_small<T, 32, MASK>(a, stream);
-    // A warp per row has no barriers and leaves a row's end to the other 31 warps of its SM, but a
-    // row takes it eight times as long: it wins once there are about as many rows as granules in
-    // one. bfloat16, 8 alternatives, warp against CTA in us: 2048 x 8000 15 and 25, 592 x 8000 12 and 9;
-    // 8192 x 32,000 123 and 152, 1024 x 32,000 29 and 25; 16,384 x 1500 40 and 209, 148 x 1500 8.4 and 8.3.
+    // A warp per row has no barriers and its row's end is hidden by the other 31 warps of its SM, but
+    // a row takes it eight times as long: it wins once there are about as many rows as granules in
+    // one. bfloat16, 8 alternatives, warp against CTA in us: 2048 x 8000 15 and 25, 592 x 8000 12 and
+    // 9; 8192 x 32,000 123 and 152, 1024 x 32,000 29 and 25; 16,384 x 1500 40 and 209, 148 x 1500 8.4
+    // and 8.3.
     const int granules = (int)((int64_t)a.vocab * (int)sizeof(T) / 16);
     if (a.rows >= granules && a.top <= kWarpTop) return launch<T, 32, MASK, false>(a, 1, stream);
-    // Parts of a row pay where there are CTAs to spare and the pass is long against what a part costs beyond it
-    // (CTA against the best cluster in us: 1 x 128,000 14.4 and 8.6, 64 x 128,000 15.9 and 11.6,
-    // 148 x 128,000 16.9 and 15.7, 64 x 32,000 8.3 and 8.5).
+    // Parts of a row pay where there are CTAs to spare and the pass is long against what a part costs
+    // beyond it (CTA against the best cluster in us: 1 x 128,000 14.4 and 8.6, 64 x 128,000 15.9 and
+    // 11.6, 148 x 128,000 16.9 and 15.7, 64 x 32,000 8.3 and 8.5).
     int cluster = 1;
     while (cluster < kMaxCluster && (int64_t)a.rows * cluster <= kSms && granules / cluster > 4000) cluster *= 2;
     if (cluster == 1) return launch<T, 256, MASK, false>(a, 1, stream);

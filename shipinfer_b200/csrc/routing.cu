@@ -391,9 +391,9 @@ struct PlanArgs {
 // of each expert go (after those of earlier warps, earlier CTAs and lower experts), and it walks its
 // run again in order, so that the sort is stable and no atomic decides a place. Bound by what an SM
 // issues and scatters, so by how many SMs a cluster has: 131,072 assignments of 256 experts take 273
-// us on one CTA (with a 64-bit division for each), 21 on a cluster of 8 and 14 on one of 16, the most there is; two
-// launches with the counts in memory between them could use them all, for a workspace and a second
-// launch. Equal ids by one ballot a bit: __match_any_sync took 25 us on the cluster of 8.
+// us on one CTA (with a 64-bit division for each), 21 on a cluster of 8 and 14 on one of 16, the most
+// there is; two launches with the counts in memory between them could use more SMs, for a workspace
+// and a second launch. Equal ids by one ballot a bit: __match_any_sync took 25 us on the cluster of 8.
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ PlanArgs a) {
     extern __shared__ int plan_smem[];
     __shared__ int scan[32];

@@ -23,7 +23,7 @@ __all__ = ["pack_allowed", "token_logprobs_device"]
 def pack_allowed(mask: Any) -> Any:
     """A bool mask ``[vocab]`` or ``[rows, vocab]`` as the bits :func:`token_logprobs_device`
     reads: int32 ``[words]`` or ``[rows, words]``, token ``v`` in bit ``v % 32`` of word ``v // 32``."""
-    if mask.dtype != torch.bool or mask.dim() not in (1, 2):
+    if mask.dtype != torch.bool or mask.dim() not in (1, 2) or mask.shape[-1] == 0:
         raise ValidationError(f"mask must be a bool [vocab] or [rows, vocab] tensor; got {mask.dtype} {list(mask.shape)}")
     vocab = int(mask.shape[-1])
     bits = torch.nn.functional.pad(mask, (0, -vocab % 32)).unflatten(-1, (-1, 32)).to(torch.int64)

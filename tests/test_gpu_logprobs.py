@@ -266,6 +266,25 @@ def test_other_stream_and_repeatability(cuda):
         assert all(torch.equal(a, b) for a, b in zip(again, want))
 
 
+def test_one_mask_row_and_overlapping_calls(cuda):
+    """A mask of one row in two dimensions serves every row; calls that overlap on two streams share
+    nothing."""
+    torch = cuda
+    x = scores(cuda, 700, 9000, "float16", 3)
+    mask = torch.rand(9000, device="cuda") < 0.5
+    one = token_logprobs_device(x, top=4, allowed=pack_allowed(mask))
+    two = token_logprobs_device(x, top=4, allowed=pack_allowed(mask)[None])
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(token_logprobs_device(x, top=4, allowed=pack_allowed(mask)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, one))
+
+
 def test_two_graphs_and_an_eager_call_share_nothing(cuda):
     torch = cuda
     shapes = [(3, 50257), (300, 97)]

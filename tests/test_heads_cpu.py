@@ -109,6 +109,7 @@ def test_python_refusals():
         lambda: combine_experts_device(x, torch.zeros(2, 2), torch.zeros(2, dtype=torch.int32)),
         lambda: combine_experts_device(x, torch.zeros(2, 3), torch.zeros((2, 2), dtype=torch.int32)),
         lambda: combine_experts_device(x, torch.zeros(2, 2), torch.zeros((2, 2), dtype=torch.int32), out=torch.zeros(2, 41)),
+        lambda: combine_experts_device(x, torch.zeros(2, 2, requires_grad=True), torch.zeros((2, 2), dtype=torch.int32)),
         lambda: combine_experts_device(x, torch.zeros(2, 2), torch.zeros((2, 2), dtype=torch.int32)),
     ]
     for i, call in enumerate(bad):
@@ -139,6 +140,9 @@ def test_pack_allowed(vocab):
     assert torch.equal(pack_allowed(torch.from_numpy(mask[1])), words[1])
     with pytest.raises(ValidationError):
         pack_allowed(torch.zeros(4))
+    with pytest.raises(ValidationError):
+        pack_allowed(torch.zeros(0, dtype=torch.bool))
+    assert pack_allowed(torch.zeros((0, vocab), dtype=torch.bool)).shape == (0, (vocab + 31) // 32)
 
 
 def test_definitions_on_known_answers():
