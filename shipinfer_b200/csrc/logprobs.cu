@@ -9,8 +9,7 @@
 //
 // One pass over the scores, by a warp, a CTA or a cluster of CTAs per row. Each thread keeps sums
 // relative to a logit of its own (in base 2: the hardware's exponential), which it raises only
-// when a logit is so far above it that the sums could overflow: a raise rescales them, as a
-// running maximum would at every new one. The threads' sums meet by one rescaling each.
+// when a logit is well above it: a raise rescales them, as a running maximum would at every new one. The threads' sums meet by one rescaling each.
 //
 // The alternatives come out of the same pass. It keeps each thread's largest logit, and a 16-bit
 // mark for each run of granules that the thread read: the upper half of the largest logit there. A
@@ -368,12 +367,16 @@ struct Running {
             h2.x = __fmaf_rn(e, y, h2.x);
         }
     }
-    // a stage; returns its largest logit
-    __device__ __forceinline__ float take(const uint4 (&u)[kUnroll], float scale, float headroom) {
+    // a stage; returns its largest logit. A row's first one: the warp's largest is every lane's
+    // reference, which few later logits are well above (with each lane's own, 4096 rows of 128,256
+    // bfloat16 scores took 17 us more).
+    __device__ __forceinline__ float take(const uint4 (&u)[kUnroll], float scale, float headroom, bool first) {
         const float top = Granule<T>::largest(u);
         best = fmaxf(best, top);
-        if (__builtin_expect(!(top <= limit), 0)) {
-            raise(top, scale, headroom);
+        float lead = top;
+        if (first) lead = from_order_bits(__reduce_max_sync(0xffffffffu, order_bits(top)));
+        if (__builtin_expect(!(lead <= limit), 0)) {
+            raise(lead, scale, headroom);
             if (limit != limit) {
 #pragma unroll 1
                 for (int k = 0; k < kUnroll; ++k) {
@@ -760,7 +763,7 @@ __device__ __noinline__ void finish(const Args& a, Shared<THREADS>& g, const Wal
 //
 // Bound by issue slots and the exponential unit, with the memory close behind: 231 instructions for
 // a thread's stage of 32 bfloat16 scores, 32 of them exponentials, of which an SM starts 16 a clock.
-// 4096 rows of 128,256 bfloat16 scores take 176 us without alternatives and 206 with 20 of them,
+// 4096 rows of 128,256 bfloat16 scores take 177 us without alternatives and 207 with 20 of them,
 // 2048 rows of float32 170; the scores alone take 161 at the memory's 6.55 TB/s. Dropped, each with
 // 20 alternatives against the kernel of its time: loads into registers, a bound's holders read again
 // whole (276 us); stages half as long (241 against 218), three CTAs of three stages (221), CTAs of 128
@@ -893,7 +896,7 @@ __global__ void __launch_bounds__(kCta<THREADS>, 1024 / kCta<THREADS>) logprobs_
                 for (int k = 0; k < kUnroll; ++k) u[k] = done + k * THREADS + tid < granules ? covered(k) : Granule<T>::empty();
             }
             if (MASK) __syncwarp();  // and this stage's are read before the next copies replace them
-            const float top = sums.take(u, a.scale, a.headroom);
+            const float top = sums.take(u, a.scale, a.headroom, k0 == 0);
             copy_stage(slot);
             slot = slot == (kStages - 1) * kStage ? 0 : slot + kStage;
             marked = k0 & ((1 << per) - 1) ? fmaxf(marked, top) : top;
@@ -1195,10 +1198,12 @@ Status launch_token_logprobs(const void* logits, int dtype, int rows, int vocab,
                              float temperature, int top, float* logprobs, float* entropy, float* top_logprobs,
                              int64_t* top_ids, cudaStream_t stream) {
     const float scale = 1.44269504088896f / temperature;
-    // The headroom is 40 in base 2, and at most twice that once reference + headroom is rounded:
-    // sums of 2^25 terms of up to 2^80, and of y times as much, stay finite.
+    // The headroom is 4 in base 2, and at most twice that once reference + headroom is rounded. More
+    // would still not overflow, but a lone high logit would have its y 2^y summed as a large number
+    // that the reference's move takes away again, and the entropy of a sure row is what is left: at
+    // 40 it was off by 40 roundings. Less would raise the reference more often for nothing.
     const Args a{logits, rows, vocab, row_stride, tokens, n_tokens, allowed, allowed_stride, 1.f / temperature, scale,
-                 40.f / scale, top, logprobs, entropy, top_logprobs, top_ids};
+                 4.f / scale, top, logprobs, entropy, top_logprobs, top_ids};
     const cudaError_t e = dtype == SHIPK_DTYPE_F32   ? launch<float>(a, stream)
                           : dtype == SHIPK_DTYPE_F16 ? launch<__half>(a, stream)
                                                      : launch<__nv_bfloat16>(a, stream);

@@ -154,6 +154,22 @@ def test_many_rows_of_middling_length(cuda, dtype):
         check(torch, x, tokens, top=1, allowed=allowed[3])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize(("rows", "vocab"), [(24, 200), (24, 5003), (900, 5003), (24, 60000)])
+def test_entropy_of_sure_rows(cuda, rows, vocab, dtype):
+    """One logit far above the rest, early or late in the row: the entropy is small and has to be
+    small. A thread's reference is at most 8 (in base 2) below its largest logit, whose y 2^y then has three
+    roundings of 8 and as many when the reference moves up, 48 u ln 2 together; log S and the
+    quotient add a few u, the other terms (at most 1e-3 of the sum) nothing to speak of: 48 u."""
+    rng = np.random.default_rng(vocab)
+    x = rng.normal(0.0, 0.3, (rows, vocab)).astype(np.float32)
+    x[np.arange(rows), rng.integers(0, vocab, rows)] = rng.uniform(20, 60, rows)
+    x = cuda.from_numpy(x).to(getattr(cuda, dtype)).cuda()
+    got = token_logprobs_device(x)[1].double().cpu().numpy()
+    want = _heads.logprobs64(x.double().cpu().numpy())[1]
+    assert (np.abs(got - want) <= 48 * _heads.EPS32 + bound(vocab, 0.0) * want).all()
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_rows_that_follow_one_another(cuda, dtype):
     """Several long rows for each CTA: a row's copies begin while the one before is ranked."""
