@@ -235,7 +235,8 @@ SHIPK_API int shipk_mask_area(const float* rows, int candidates, int stride, int
  * words apart (0: one mask for every row), or NULL: all. A logit of -inf is not allowed either,
  * whatever its bit; values at cleared bits, NaN and infinities among them, do not matter. A row
  * with nothing allowed has log-probabilities -inf, entropy 0 and no alternatives. A NaN or +inf
- * among the allowed makes the row's log-probabilities and entropy NaN; a NaN is no alternative.
+ * among the allowed makes the row's log-probabilities and entropy NaN; a NaN is no alternative. No
+ * log-probability is above 0 and no entropy below it, by a rounding either.
  * Sums are held in 32 bits relative to the maximum. top <= 64 (else SHIPK_ERANGE) and <= vocab;
  * temperature in [1e-6, 1e6]. tokens and logprobs may be NULL when n_tokens is 0, top_ids and
  * top_logprobs when top is 0. Outputs must not overlap inputs. One launch, no workspace. */

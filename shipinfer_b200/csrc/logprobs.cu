@@ -710,7 +710,9 @@ __device__ __forceinline__ void choose(Shared<THREADS>& g, const Row<T, MASK>& r
     rank<T, MASK, THREADS>(g, r, run, wanted, tid, t);
 }
 
-// The row's results from its sums and its alternatives' keys.
+// The row's results from its sums and its alternatives' keys. The sums' own roundings (a reference's y
+// is not exactly 0, nor is it the row's maximum) leave a sure row on either side of 0, by one step: what
+// the definition bounds by 0 is cut off there, which brings no value further from the definition.
 template <typename T, bool MASK, int THREADS>
 __device__ __forceinline__ void write_row(const Args& a, const Row<T, MASK>& r, int64_t row, const Part& p,
                                           const uint64_t* chosen, int tid) {
@@ -718,9 +720,13 @@ __device__ __forceinline__ void write_row(const Args& a, const Row<T, MASK>& r, 
     const float log_s = empty ? 0.f : logf(p.s);
     auto logprob = [&](float x) {
         if (empty || (x == -INFINITY && p.s == p.s)) return -INFINITY;
-        return (x - p.m) * a.inv_t - log_s;  // NaN where S is
+        const float v = (x - p.m) * a.inv_t - log_s;
+        return v > 0.f ? 0.f : v;  // NaN where S is
     };
-    if (tid == 0) a.entropy[row] = empty ? 0.f : log_s - 0.693147180559945f * (p.h / p.s);
+    if (tid == 0) {
+        const float v = empty ? 0.f : log_s - 0.693147180559945f * (p.h / p.s);
+        a.entropy[row] = v < 0.f ? 0.f : v;
+    }
     for (int j = tid; j < a.n_tokens; j += THREADS) {
         const int64_t t = a.tokens[row * a.n_tokens + j];
         a.logprobs[row * a.n_tokens + j] = t < 0 ? 0.f : t >= a.vocab ? NAN : logprob(r.logit((int)t));
