@@ -239,7 +239,8 @@ SHIPK_API int shipk_mask_area(const float* rows, int candidates, int stride, int
  * log-probability is above 0 and no entropy below it, by a rounding either.
  * Sums are held in 32 bits relative to the maximum. top <= 64 (else SHIPK_ERANGE) and <= vocab;
  * temperature in [1e-6, 1e6]. tokens and logprobs may be NULL when n_tokens is 0, top_ids and
- * top_logprobs when top is 0. Outputs must not overlap inputs. One launch, no workspace. */
+ * top_logprobs when top is 0. Outputs must overlap neither inputs nor one another (SHIPK_EINVAL).
+ * One launch, no workspace. */
 SHIPK_API int shipk_token_logprobs(const void* logits, int dtype, int rows, int vocab, int64_t row_stride,
                                    const int64_t* tokens, int n_tokens, const uint32_t* allowed,
                                    int64_t allowed_stride, float temperature, int top, float* logprobs,
@@ -265,7 +266,8 @@ SHIPK_API int shipk_token_logprobs(const void* logits, int dtype, int rows, int 
  * 0), times `scale`. Past the last expert that can be chosen: id -1, weight 0. Mask an expert
  * with -inf: a type's lowest finite value is a number, which a bias can still lift.
  * experts <= 1024, top_k <= 32, groups <= 32 (else SHIPK_ERANGE); top_k <= experts, groups
- * divides experts, 1 <= top_groups <= groups. Outputs must not overlap inputs. One launch. */
+ * divides experts, 1 <= top_groups <= groups. Outputs must overlap neither inputs nor one another
+ * (SHIPK_EINVAL). One launch. */
 SHIPK_API int shipk_route_experts(const void* logits, int dtype, int rows, int experts, int64_t row_stride,
                                   const float* bias, int top_k, int scores, int groups, int top_groups,
                                   int group_score, int renormalise, float scale, float* weights,
@@ -277,7 +279,8 @@ SHIPK_API int shipk_route_experts(const void* logits, int dtype, int rows, int e
  * offsets[experts]; what shipk_crop_u8 reads as boxes in this order is each expert's batch.
  * slots (device int32 [rows, k]): the place of each assignment, -1 where the id is outside
  * [0, experts) (nothing chosen). experts <= 1024, rows * k <= 2^31 - 2^16 (else SHIPK_ERANGE). Outputs
- * must not overlap the input. One launch, no workspace, the same result every time. */
+ * must overlap neither the input nor one another (SHIPK_EINVAL). One launch, no workspace, the
+ * same result every time. */
 SHIPK_API int shipk_plan_experts(const int32_t* ids, int rows, int k, int experts, int32_t* order,
                                  int32_t* slots, int32_t* offsets, void* stream);
 
@@ -285,7 +288,7 @@ SHIPK_API int shipk_plan_experts(const int32_t* ids, int rows, int k, int expert
  * bits in the order of j and rounded once to `dtype` (F32, F16 or BF16). in: device [n_in, width],
  * rows `row_stride` elements apart, in the plan's order; weights: device float [rows, k]; slots:
  * device int32 [rows, k], an assignment whose slot is outside [0, n_in) adds nothing, whatever
- * its weight; out: device [rows, width]. Outputs must not overlap inputs. One launch. */
+ * its weight; out: device [rows, width], which must overlap no input (SHIPK_EINVAL). One launch. */
 SHIPK_API int shipk_combine_experts(const void* in, int dtype, int n_in, int64_t row_stride,
                                     const float* weights, const int32_t* slots, int rows, int k,
                                     int width, void* out, void* stream);

@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <new>
@@ -598,6 +599,42 @@ int element_bytes(int dtype) {
     return dtype == SHIPK_DTYPE_F32 ? 4 : dtype == SHIPK_DTYPE_F16 || dtype == SHIPK_DTYPE_BF16 ? 2 : 0;
 }
 
+// A tensor's memory: rows of `bytes`, `stride` bytes apart.
+struct Extent {
+    const char* name;
+    const void* at;
+    int64_t rows, bytes, stride;
+};
+// in bytes, without an overflow: past the address space every length and stride means the same
+int64_t in_bytes(int64_t elements, int size) { return std::min(elements, (int64_t)1 << 57) * size; }
+Extent dense(const char* name, const void* at, int64_t elements, int size) {
+    return {name, at, 1, in_bytes(elements, size), 0};
+}
+Extent spread(const char* name, const void* at, int64_t rows, int64_t cols, int64_t stride, int size) {
+    return {name, at, rows, in_bytes(cols, size), in_bytes(stride, size)};
+}
+
+// Whether a result (dense) shares a byte with another tensor's rows; it may lie between them.
+bool meets(const Extent& t, const Extent& result) {
+    if (!t.at || !result.at || t.rows < 1 || t.bytes < 1 || result.bytes < 1) return false;
+    const int64_t lo = (int64_t)(reinterpret_cast<uintptr_t>(result.at) - reinterpret_cast<uintptr_t>(t.at));
+    const int64_t hi = lo + result.bytes;  // the result's bytes, from the tensor's first
+    if (t.stride == 0 || lo < t.bytes) return lo < t.bytes && hi > 0;
+    const int64_t row = (lo - t.bytes) / t.stride + 1;  // the first that ends behind the result's start
+    return row < t.rows && row * t.stride < hi;
+}
+
+// A kernel reads its inputs while it writes its results, some of them twice.
+int check_apart(const char* who, std::initializer_list<Extent> inputs, std::initializer_list<Extent> results) {
+    for (const Extent* r = results.begin(); r != results.end(); ++r) {
+        for (const Extent& t : inputs)
+            if (meets(t, *r)) return fail(SHIPK_EINVAL, "%s: %s overlaps %s", who, r->name, t.name);
+        for (const Extent* o = results.begin(); o != r; ++o)
+            if (meets(*o, *r)) return fail(SHIPK_EINVAL, "%s: %s overlaps %s", who, r->name, o->name);
+    }
+    return SHIPK_OK;
+}
+
 // A device pointer on a boundary of its elements: a kernel's load from any other address faults.
 int check_elements(const void* ptr, int bytes, const char* who, const char* name) {
     const int rc = check_device_ptr(ptr, who, name);
@@ -626,7 +663,15 @@ int shipk_token_logprobs(const void* logits, int dtype, int rows, int vocab, int
     if (!(temperature >= 1e-6f && temperature <= 1e6f))
         return fail(SHIPK_EINVAL, "%s: temperature %g is outside 1e-6..1e6", who, (double)temperature);
     if (rows == 0) return SHIPK_OK;
-    int rc;
+    int rc = check_apart(who,
+                         {spread("logits", logits, rows, vocab, row_stride, size),
+                          dense("tokens", tokens, (int64_t)rows * n_tokens, 8),
+                          spread("allowed", allowed, rows, (vocab + 31) / 32, allowed_stride, 4)},
+                         {dense("logprobs", logprobs, (int64_t)rows * n_tokens, 4),
+                          dense("entropy", entropy, rows, 4),
+                          dense("top_logprobs", top_logprobs, (int64_t)rows * top, 4),
+                          dense("top_ids", top_ids, (int64_t)rows * top, 8)});
+    if (rc) return rc;
     if ((rc = check_elements(logits, size, who, "logits"))) return rc;
     if ((rc = check_elements(entropy, 4, who, "entropy"))) return rc;
     if (n_tokens > 0) {
@@ -666,7 +711,12 @@ int shipk_route_experts(const void* logits, int dtype, int rows, int experts, in
         return fail(SHIPK_EINVAL, "%s: group_score %d is neither max nor top2", who, group_score);
     if (row_stride < 0) return fail(SHIPK_EINVAL, "%s: row_stride is negative", who);
     if (rows == 0) return SHIPK_OK;
-    int rc;
+    int rc = check_apart(who,
+                         {spread("logits", logits, rows, experts, row_stride, size),
+                          dense("bias", bias, experts, 4)},
+                         {dense("weights", weights, (int64_t)rows * top_k, 4),
+                          dense("ids", ids, (int64_t)rows * top_k, 4)});
+    if (rc) return rc;
     if ((rc = check_elements(logits, size, who, "logits"))) return rc;
     if (bias && (rc = check_elements(bias, 4, who, "bias"))) return rc;
     if ((rc = check_elements(weights, 4, who, "weights"))) return rc;
@@ -683,9 +733,13 @@ int shipk_plan_experts(const int32_t* ids, int rows, int k, int experts, int32_t
     if (rows < 0 || k < 1) return fail(SHIPK_EINVAL, "%s: rows %d or k %d is out of range", who, rows, k);
     if (experts < 1) return fail(SHIPK_EINVAL, "%s: %d experts", who, experts);
     if (experts > kMaxExperts) return fail(SHIPK_ERANGE, "%s: %d experts are above %d", who, experts, kMaxExperts);
-    if ((int64_t)rows * k > 0x7fffffff - 0x10000)
+    const int64_t pairs = (int64_t)rows * k;
+    if (pairs > 0x7fffffff - 0x10000)
         return fail(SHIPK_ERANGE, "%s: %d rows of %d assignments are above 2^31 - 2^16", who, rows, k);
-    int rc;
+    int rc = check_apart(who, {dense("ids", ids, pairs, 4)},
+                         {dense("order", order, pairs, 4), dense("slots", slots, pairs, 4),
+                          dense("offsets", offsets, (int64_t)experts + 1, 4)});
+    if (rc) return rc;
     if ((rc = check_elements(offsets, 4, who, "offsets"))) return rc;
     if (rows > 0) {
         if ((rc = check_elements(ids, 4, who, "ids"))) return rc;
@@ -705,7 +759,12 @@ int shipk_combine_experts(const void* in, int dtype, int n_in, int64_t row_strid
         return fail(SHIPK_EINVAL, "%s: rows %d, results %d, k %d or width %d is out of range", who, rows, n_in, k, width);
     if (row_stride < 0) return fail(SHIPK_EINVAL, "%s: row_stride is negative", who);
     if (rows == 0 || width == 0) return SHIPK_OK;
-    int rc;
+    int rc = check_apart(who,
+                         {spread("in", in, n_in, width, row_stride, size),
+                          dense("weights", weights, (int64_t)rows * k, 4),
+                          dense("slots", slots, (int64_t)rows * k, 4)},
+                         {dense("out", out, (int64_t)rows * width, size)});
+    if (rc) return rc;
     if (n_in > 0 && (rc = check_elements(in, size, who, "in"))) return rc;
     if ((rc = check_elements(weights, 4, who, "weights"))) return rc;
     if ((rc = check_elements(slots, 4, who, "slots"))) return rc;

@@ -498,7 +498,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
             if (id[q] < a.experts && lane == __ffs(peers) - 1) mine[id[q]] += __popc(peers);
             __syncwarp();
             if (i < hi) a.slots[i] = place;
-            if (place >= 0) a.order[place] = (int)((unsigned)i / (unsigned)a.k);
+            // below pairs always, but where another stream's call changes the ids between their two readings
+            if ((unsigned)place < (unsigned)a.pairs) a.order[place] = (int)((unsigned)i / (unsigned)a.k);
         }
     }
     for (int64_t i = (int64_t)kept + rank * threads + tid; i < a.pairs; i += ranks * threads) a.order[i] = -1;

@@ -57,7 +57,8 @@ def token_logprobs_device(
             -inf, has probability 0; the values at cleared bits do not matter.
         temperature: divides the scores, 1e-6 to 1e6.
         logprobs, entropy, top_logprobs, top_ids: optional results to fill: float32 of the tokens'
-            shape, ``[rows]``, ``[rows, top]`` and int64 ``[rows, top]``.
+            shape, ``[rows]``, ``[rows, top]`` and int64 ``[rows, top]``, apart from the inputs and
+            from one another.
         stream: CUDA stream handle; torch's current stream when ``None``.
 
     Returns:

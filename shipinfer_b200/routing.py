@@ -58,7 +58,8 @@ def route_experts_device(
             expert ("max") or the sum of their two best ("top2").
         renormalise: divide the chosen scores by their sum.
         scale: multiplies the weights.
-        weights, ids: optional results to fill: float32 and int32 ``[rows, top_k]``.
+        weights, ids: optional results to fill: float32 and int32 ``[rows, top_k]``, apart from the
+            inputs and from each other.
         stream: CUDA stream handle; torch's current stream when ``None``.
 
     Returns:
@@ -111,7 +112,7 @@ def plan_experts_device(
             ``[0, experts)`` is nobody's.
         experts: how many there are, up to 1024.
         order, slots, offsets: optional results to fill: int32 ``[rows * k]``, ``[rows, k]`` and
-            ``[experts + 1]``.
+            ``[experts + 1]``, apart from the ids (which are read twice) and from one another.
         stream: CUDA stream handle; torch's current stream when ``None``.
 
     Returns:
@@ -160,7 +161,7 @@ def combine_experts_device(
             places of the plan; rows may lie apart.
         weights: CUDA float32 ``[r, k]``; slots: CUDA int32 ``[r, k]``. A slot outside ``[0, n)``
             adds nothing, whatever its weight.
-        out: optional result to fill, ``[r, width]`` of the rows' type.
+        out: optional result to fill, ``[r, width]`` of the rows' type, apart from the inputs.
         stream: CUDA stream handle; torch's current stream when ``None``.
 
     Returns:
