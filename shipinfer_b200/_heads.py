@@ -28,8 +28,14 @@ def element_code(t: Any, name: str) -> int:
 
 
 def small(value: Any, name: str) -> int:
-    """An integer that the C ABI takes as 32 bits: one that does not fit would arrive as another."""
-    value = int(value)
+    """A whole number that the C ABI takes as 32 bits: one that does not fit would arrive as another."""
+    given = value
+    try:
+        value = int(given)
+    except (TypeError, ValueError, OverflowError):
+        value = None
+    if value is None or value != given:
+        raise ValidationError(f"{name} must be a whole number; got {given!r}")
     if not -(1 << 31) <= value < 1 << 31:
         raise ConfigurationError(f"{name} {value} does not fit in 32 bits")
     return value
