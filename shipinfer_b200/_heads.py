@@ -7,6 +7,7 @@ from contextlib import nullcontext
 from typing import Any
 
 import torch
+from torch.autograd import forward_ad
 
 from shipinfer_b200 import _native
 from shipinfer_b200.errors import ConfigurationError, ValidationError
@@ -41,6 +42,15 @@ def small(value: Any, name: str) -> int:
     return value
 
 
+def refuse_gradient(t: Any, name: str) -> None:
+    """A result without its gradient or tangent would pass for one that does not depend on `t`."""
+    # outside every dual level (-1), where no tensor has a tangent, unpack_dual's 0.5 us are spared
+    if (t.requires_grad and torch.is_grad_enabled()) or (
+        getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
+    ):
+        raise ValidationError(f"{name} asks for a gradient; this call computes none (use no_grad, detach or the primal)")
+
+
 def check_matrix(t: Any, name: str) -> tuple[int, int]:
     """A score or result matrix: its rows may lie apart, the values within one may not."""
     if t.dim() != 2:
@@ -50,8 +60,7 @@ def check_matrix(t: Any, name: str) -> tuple[int, int]:
         raise ConfigurationError(f"{name}: {rows} rows of {cols} do not fit in 32 bits")
     if cols > 1 and rows > 0 and t.stride(1) != 1:
         raise ValidationError(f"{name}: the values of a row must be adjacent; strides {tuple(t.stride())}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValidationError(f"{name} asks for a gradient; this call computes none (use no_grad or detach)")
+    refuse_gradient(t, name)
     return rows, cols
 
 
@@ -61,8 +70,7 @@ def check_dense(t: Any, name: str, dtype: Any, shape: tuple[int, ...]) -> None:
             f"{name} must be a contiguous {str(dtype).removeprefix('torch.')} {list(shape)} CUDA tensor; "
             f"got {t.dtype} {list(t.shape)}"
         )
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValidationError(f"{name} asks for a gradient; this call computes none (use no_grad or detach)")
+    refuse_gradient(t, name)
 
 
 def check_device(*tensors: Any) -> int:

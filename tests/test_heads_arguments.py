@@ -9,7 +9,7 @@ import torch
 
 from shipinfer_b200 import ConfigurationError, ValidationError, _heads
 from shipinfer_b200.logprobs import token_logprobs_device
-from shipinfer_b200.routing import plan_experts_device, route_experts_device
+from shipinfer_b200.routing import combine_experts_device, plan_experts_device, route_experts_device
 
 
 @pytest.mark.parametrize("value", [2.7, "3", None, float("nan"), float("inf"), np.float32(1.5)])
@@ -31,3 +31,39 @@ def test_whole_numbers_of_any_kind():
     with pytest.raises(ConfigurationError, match="does not fit"):
         _heads.small(1 << 31, "n")
     assert _heads.small(-(1 << 31), "n") == -(1 << 31)
+
+
+def test_gradients_and_tangents():
+    """Scores, weights and biases that carry a gradient or a forward-mode tangent: the results would lose it."""
+    x, w, slots = torch.zeros(3, 40), torch.zeros(3, 2), torch.zeros((3, 2), dtype=torch.int32)
+    bias = torch.zeros(40)
+
+    def calls(carries):
+        return [
+            (lambda: token_logprobs_device(carries(x)), "logits"),
+            (lambda: token_logprobs_device(x, entropy=carries(torch.zeros(3))), "entropy"),
+            (lambda: route_experts_device(carries(x), top_k=2), "logits"),
+            (lambda: route_experts_device(x, top_k=2, bias=carries(bias)), "bias"),
+            (lambda: combine_experts_device(carries(x), w, slots), "rows"),
+            (lambda: combine_experts_device(x, carries(w), slots), "weights"),
+        ]
+
+    def refused(carries):
+        for call, name in calls(carries):
+            with pytest.raises(ValidationError, match=f"^{name} asks for a gradient"):
+                call()
+
+    def passed_over(carries):  # to the next check, the device's
+        for call, _ in calls(carries):
+            with pytest.raises(ValidationError, match="must be CUDA tensors"):
+                call()
+
+    refused(lambda t: t.clone().requires_grad_())
+    with torch.no_grad():
+        passed_over(lambda t: t.clone().requires_grad_())
+    with torch.autograd.forward_ad.dual_level():
+        refused(lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+        passed_over(lambda t: torch.autograd.forward_ad.unpack_dual(
+            torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))).primal)
+        passed_over(lambda t: t)
+    passed_over(lambda t: t)
