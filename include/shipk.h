@@ -263,8 +263,8 @@ SHIPK_API int shipk_token_logprobs(const void* logits, int dtype, int rows, int 
  * (group_score; ties to the lower group) can be chosen. The top_k largest choices, ties to the
  * lower expert, go to ids (device int32 [rows, top_k], best first); weights (device float) are
  * their scores, without the bias, divided by their sum when `renormalise` (0 where that sum is
- * 0), times `scale`. Past the last expert that can be chosen: id -1, weight 0. Mask an expert
- * with -inf: a type's lowest finite value is a number, which a bias can still lift.
+ * 0), times `scale`, which is finite. Past the last expert that can be chosen: id -1, weight 0.
+ * Mask an expert with -inf: a type's lowest finite value is a number, which a bias can still lift.
  * experts <= 1024, top_k <= 32, groups <= 32 (else SHIPK_ERANGE); top_k <= experts, groups
  * divides experts, 1 <= top_groups <= groups. Outputs must overlap neither inputs nor one another
  * (SHIPK_EINVAL). One launch. */

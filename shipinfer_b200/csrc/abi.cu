@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -709,6 +710,7 @@ int shipk_route_experts(const void* logits, int dtype, int rows, int experts, in
         return fail(SHIPK_EINVAL, "%s: scores %d is neither softmax nor sigmoid", who, scores);
     if (group_score != SHIPK_GROUP_MAX && group_score != SHIPK_GROUP_TOP2)
         return fail(SHIPK_EINVAL, "%s: group_score %d is neither max nor top2", who, group_score);
+    if (!std::isfinite(scale)) return fail(SHIPK_EINVAL, "%s: scale %g is not finite", who, (double)scale);
     if (row_stride < 0) return fail(SHIPK_EINVAL, "%s: row_stride is negative", who);
     if (rows == 0) return SHIPK_OK;
     int rc = check_apart(who,

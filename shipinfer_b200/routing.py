@@ -57,7 +57,7 @@ def route_experts_device(
             runs (up to 32) and only the ``top_groups`` best can be chosen from, by their best
             expert ("max") or the sum of their two best ("top2").
         renormalise: divide the chosen scores by their sum.
-        scale: multiplies the weights.
+        scale: multiplies the weights; finite in float32.
         weights, ids: optional results to fill: float32 and int32 ``[rows, top_k]``, apart from the
             inputs and from each other.
         stream: CUDA stream handle; torch's current stream when ``None``.

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from shipinfer_b200 import ConfigurationError, ValidationError, _heads
+from shipinfer_b200 import ConfigurationError, ValidationError, _heads, _native
 from shipinfer_b200.logprobs import token_logprobs_device
 from shipinfer_b200.routing import combine_experts_device, plan_experts_device, route_experts_device
 
@@ -161,3 +161,13 @@ I32, I64 = torch.int32, torch.int64
 def test_each_refusal_by_its_own_check(call, text):
     with pytest.raises(ValidationError, match=text):
         call()
+
+
+@pytest.mark.parametrize("scale", [float("inf"), -float("inf"), float("nan"), 1e39])
+def test_scales_that_are_not_finite(scale):
+    """Times such a scale, the weight 0 of an expert that is not there would be NaN."""
+    lib = _native.lib()
+    code = lib.shipk_route_experts(None, 0, 0, 8, 8, None, 2, 0, 1, 1, 0, 1, scale, None, None, None)
+    assert code == _native.EINVAL and "scale" in _native.last_error()
+    for fine in (0.0, -2.5, 3.4e38):
+        assert lib.shipk_route_experts(None, 0, 0, 8, 8, None, 2, 0, 1, 1, 0, 1, fine, None, None, None) == 0
