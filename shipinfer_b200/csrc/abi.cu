@@ -114,6 +114,21 @@ cudaError_t ensure_smem_attr(const void* func, int bytes) {
     return e;
 }
 
+// SMs of the current device, asked for once.
+int sm_count() {
+    static std::mutex mu;
+    static std::map<int, int> cache;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = cache.find(dev);
+    if (it != cache.end()) return it->second;
+    int sms = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+    cache[dev] = sms;
+    return sms;
+}
+
 }  // namespace shipk
 
 using namespace shipk;

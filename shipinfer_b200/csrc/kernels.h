@@ -122,6 +122,9 @@ Status launch_normalise_check(float mean, float stdv, unsigned long long* result
 // Opt a kernel into more than 48 KB of dynamic shared memory on the current device, once.
 cudaError_t ensure_smem_attr(const void* func, int bytes);
 
+// SMs of the current device.
+int sm_count();
+
 // Taps of the letterbox resize along one axis, computed on the host with the kernel's own
 // arithmetic; used to decide which source rows a host-frame call must upload.
 void letterbox_rows_needed(int src_h, int new_h, unsigned char* needed);

@@ -35,8 +35,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <map>
-#include <mutex>
 #include <tuple>
 #include <type_traits>
 
@@ -1123,20 +1121,6 @@ const char* plan_letterbox(const FrameView* frames, int n, void* out, int dst_h,
     p.table_off = warps * p.warp_bytes;
     plan->smem = p.table_off + p.ntables * p.table_bytes;
     return nullptr;
-}
-
-int sm_count() {
-    static std::mutex mu;
-    static std::map<int, int> cache;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> lock(mu);
-    auto it = cache.find(dev);
-    if (it != cache.end()) return it->second;
-    int sms = 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
-    cache[dev] = sms;
-    return sms;
 }
 
 template <typename OutT, int VEC, bool NV12, int CTAS>

@@ -1135,7 +1135,6 @@ __global__ void __launch_bounds__(kWarpCta) logprobs_small_kernel(const __grid_c
     }
 }
 
-constexpr int kSms = 148;
 constexpr int kWarpTop = 20;  // alternatives that 32 threads' maxima bound
 
 template <typename T, int THREADS, bool MASK, bool CLUSTER>
@@ -1148,7 +1147,8 @@ cudaError_t launch(const Args& a, int cluster, cudaStream_t stream) {
     cudaLaunchConfig_t config{};
     // as many CTAs as run at once, which walk over the rows; with clusters, all of them
     config.gridDim = CLUSTER ? dim3((unsigned)(a.rows * cluster))
-                             : dim3((unsigned)std::min<int64_t>(((int64_t)a.rows + kRows - 1) / kRows, kSms * (1024 / kThreads)));
+                             : dim3((unsigned)std::min<int64_t>(((int64_t)a.rows + kRows - 1) / kRows,
+                                                                (int64_t)sm_count() * (1024 / kThreads)));
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = ring;
     config.stream = stream;
@@ -1186,8 +1186,9 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
     // Parts of a row pay where there are CTAs to spare and the pass is long against what a part costs
     // beyond it (CTA against the best cluster in us: 1 x 128,000 14.4 and 8.6, 64 x 128,000 15.9 and
     // 11.6, 148 x 128,000 16.9 and 15.7, 64 x 32,000 8.3 and 8.5).
+    const int sms = sm_count();
     int cluster = 1;
-    while (cluster < kMaxCluster && (int64_t)a.rows * cluster <= kSms && granules / cluster > 4000) cluster *= 2;
+    while (cluster < kMaxCluster && (int64_t)a.rows * cluster <= sms && granules / cluster > 4000) cluster *= 2;
     if (cluster == 1) return launch<T, 256, MASK, false>(a, 1, stream);
     return launch<T, 256, MASK, true>(a, cluster, stream);
 }
