@@ -559,9 +559,9 @@ __device__ __noinline__ void choose_slowly(Shared<THREADS>& g, Row<T, MASK> r, R
 // each turn a tighter one: what is above it is collected from the whole row. Then the first that equal it,
 // found in the row's order until there are enough. False if more is above the last bound than the group can
 // hold. One or two readings of the row more, where one for each alternative took (float16, 20 alternatives,
-// logits of -log(id) and noise) 64 x 128,256 from 52 to 223 us, 8192 x 32,000 from 235 to 1515; ordinary rows 13
-// and 172. The row's main pass feels its registers: the second loop is unrolled by 2 only (4 as the compiler has it:
-// 1% on ordinary rows of 128,256).
+// logits of -log(id) and noise) 64 x 128,256 from 45 to 223 us and 8192 x 32,000 from 230 to 1515; ordinary rows
+// take 13 and 172. The row's main pass feels this function's registers, so it is kept narrow: order bits
+// instead of keys (52 and 235 with keys), loops that are not unrolled further. With that 4096 x 128,256 bfloat16 take 209 us, 207 without this way.
 template <typename T, bool MASK, int THREADS>
 __device__ __noinline__ bool collect_tighter(Shared<THREADS>& g, Row<T, MASK> r, Run<T, MASK, THREADS> run,
                                              int wanted, int tid, uint32_t t) {
@@ -572,13 +572,16 @@ __device__ __noinline__ bool collect_tighter(Shared<THREADS>& g, Row<T, MASK> r,
         group_sync<THREADS>();
         const int n = min(g.collected, kHold);
         if (n >= wanted) {
+            if (tid == 0) g.bound = ~0u;
+            group_sync<THREADS>();
+            auto held = [&](int i) { return (uint32_t)(g.keys[i] >> 32); };
 #pragma unroll 1
             for (int i = tid; i < n; i += THREADS) {
-                const uint64_t k = g.keys[i];
+                const uint32_t k = held(i);
                 int better = 0;
-#pragma unroll 2
-                for (int j = 0; j < n; ++j) better += g.keys[j] > k;
-                if (better == wanted - 1) g.bound = (uint32_t)(k >> 32);
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) better += held(j) > k;
+                if (better < wanted) atomicMin(&g.bound, k);
             }
             group_sync<THREADS>();
             t = g.bound;
