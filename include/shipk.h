@@ -237,10 +237,10 @@ SHIPK_API int shipk_mask_area(const float* rows, int candidates, int stride, int
  * with nothing allowed has log-probabilities -inf, entropy 0 and no alternatives. A NaN or +inf
  * among the allowed makes the row's log-probabilities and entropy NaN; a NaN is no alternative. No
  * log-probability is above 0 and no entropy below it, by a rounding either.
- * Sums are held in 32 bits relative to the maximum. top <= 64 (else SHIPK_ERANGE) and <= vocab;
- * temperature in [1e-6, 1e6]. tokens and logprobs may be NULL when n_tokens is 0, top_ids and
- * top_logprobs when top is 0. Outputs must overlap neither inputs nor one another (SHIPK_EINVAL).
- * One launch, no workspace. */
+ * Sums are held in 32 bits relative to one of the row's logits, at most 8 (in units of temperature
+ * ln 2) below its largest. top <= 64 (else SHIPK_ERANGE) and <= vocab; temperature in [1e-6, 1e6].
+ * tokens and logprobs may be NULL when n_tokens is 0, top_ids and top_logprobs when top is 0.
+ * Outputs must overlap neither inputs nor one another (SHIPK_EINVAL). One launch, no workspace. */
 SHIPK_API int shipk_token_logprobs(const void* logits, int dtype, int rows, int vocab, int64_t row_stride,
                                    const int64_t* tokens, int n_tokens, const uint32_t* allowed,
                                    int64_t allowed_stride, float temperature, int top, float* logprobs,

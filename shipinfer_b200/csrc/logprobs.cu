@@ -561,7 +561,8 @@ __device__ __noinline__ void choose_slowly(Shared<THREADS>& g, Row<T, MASK> r, R
 // hold. One or two readings of the row more, where one for each alternative took (float16, 20 alternatives,
 // logits of -log(id) and noise) 64 x 128,256 from 45 to 223 us and 8192 x 32,000 from 230 to 1515; ordinary rows
 // take 13 and 172. The row's main pass feels this function's registers, so it is kept narrow: order bits
-// instead of keys (52 and 235 with keys), loops that are not unrolled further. With that 4096 x 128,256 bfloat16 take 209 us, 207 without this way.
+// instead of keys (52 and 235 with keys), loops that are not unrolled further. With that 4096 x 128,256 bfloat16
+// take 209 us, 207 without this way.
 template <typename T, bool MASK, int THREADS>
 __device__ __noinline__ bool collect_tighter(Shared<THREADS>& g, Row<T, MASK> r, Run<T, MASK, THREADS> run,
                                              int wanted, int tid, uint32_t t) {
@@ -796,10 +797,11 @@ __device__ __noinline__ void finish(const Args& a, Shared<THREADS>& g, const Wal
 // take 4 us from a busy memory, an eighth of a row of 128,256 bfloat16 scores): it asks for them
 // when the row ends, looks at them after the next row's second stage and ranks them after its third.
 //
-// Bound by issue slots and the exponential unit, with the memory close behind: 231 instructions for
-// a thread's stage of 32 bfloat16 scores, 32 of them exponentials, of which an SM starts 16 a clock.
-// 4096 rows of 128,256 bfloat16 scores take 177 us without alternatives and 207 with 20 of them,
-// 2048 rows of float32 170; the scores alone take 161 at the memory's 6.55 TB/s. Dropped, each with
+// No unit is full: with 20 alternatives, 4096 rows of 128,256 bfloat16 scores keep the issue slots busy 69% of the
+// time, the exponential unit 61% and the memory 60% (without alternatives 70, 68 and 68), and a CTA's warps wait most
+// at the barriers of its rows' ends. A thread's stage of 32 such scores is 231 instructions, 32 of them
+// exponentials, of which an SM starts 16 a clock. These rows take 182 us without alternatives and 209 with 20 of
+// them, 2048 rows of float32 174; the scores alone take 161 at the memory's 6.55 TB/s. Dropped, each with
 // 20 alternatives against the kernel of its time: loads into registers, a bound's holders read again
 // whole (276 us); stages half as long (241 against 218), three CTAs of three stages (221), CTAs of 128
 // threads (233), two warps of a CTA that finish what eight read (212 against 214, slower for few
@@ -1164,7 +1166,10 @@ __global__ void __launch_bounds__(kWarpCta) logprobs_small_kernel(const __grid_c
     }
 }
 
-constexpr int kWarpTop = 20;  // alternatives that 32 threads' maxima bound
+// Alternatives for which the maxima of a warp's 32 threads are a bound that few scores pass: warp against CTA in us,
+// bfloat16, with 20 16,384 x 1500 53 and 230, 2048 x 8000 19 and 30, 8192 x 32,000 172 and 168; with 24 63 and 242, 23
+// and 30, 204 and 172; with 28 109 and 250, 63 and 31, 463 and 177.
+constexpr int kWarpTop = 20;
 
 template <typename T, int THREADS, bool MASK, bool CLUSTER>
 cudaError_t launch(const Args& a, int cluster, cudaStream_t stream) {
@@ -1200,6 +1205,10 @@ cudaError_t launch_small(const Args& a, cudaStream_t stream) {
 
 template <typename T, bool MASK>
 cudaError_t launch(const Args& a, cudaStream_t stream) {
+    // A row in a warp's registers: up to where two passes over them cost more than a warp's or a CTA's one over memory.
+    // 1000 scores, registers against logprobs_kernel in us: float32 64 rows, 3 alternatives 3.8 and 5.7, 4096
+    // rows 10.4 and 10.2; bfloat16 16,384 rows 29.9 and 26.4. 300 scores: 2.9 and 5.4, 5.8 and 8.1. Each alternative is a pass
+    // more, so with 20 of them 4096 x 300 takes 19.4 and 10.7, 4096 x 1000 33.5 and 13.9.
     if (a.vocab <= 32) return launch_small<T, 1, MASK>(a, stream);
     if (a.vocab <= 128) return launch_small<T, 4, MASK>(a, stream);
     if (a.vocab <= 256) return launch_small<T, 8, MASK>(a, stream);
@@ -1213,8 +1222,9 @@ cudaError_t launch(const Args& a, cudaStream_t stream) {
     const int granules = (int)((int64_t)a.vocab * (int)sizeof(T) / 16);
     if (a.rows >= granules && a.top <= kWarpTop) return launch<T, 32, MASK, false>(a, 1, stream);
     // Parts of a row pay where there are CTAs to spare and the pass is long against what a part costs
-    // beyond it (CTA against the best cluster in us: 1 x 128,000 14.4 and 8.6, 64 x 128,000 15.9 and
-    // 11.6, 148 x 128,000 16.9 and 15.7, 64 x 32,000 8.3 and 8.5).
+    // beyond it. In us, 1, 2, 4 and 8 parts as far as the rule's border is lowered, 8 alternatives, bfloat16: 64 x 128,000
+    // 16.2 and 11.8 (4 parts), 1 x 128,000 15.1, 9.2 (4) and 8.5 (8); 64 x 50,257 11.0, 10.3 (2) and 10.0 (4); 64 x 32,000
+    // 8.1 and 8.5 (2). More CTAs than SMs: 148 x 50,257 11.5 and 12.7 (2), 148 x 128,000 16.9 and 15.7.
     const int sms = sm_count();
     int cluster = 1;
     while (cluster < kMaxCluster && (int64_t)a.rows * cluster <= sms && granules / cluster > 4000) cluster *= 2;
