@@ -641,7 +641,7 @@ Status launch_plan(const int32_t* ids, int rows, int k, int experts, int32_t* or
     config.attrs = &attr;
     config.numAttrs = 1;
     // a cluster once one CTA's warps would walk for long (CTA against cluster of 16 in us, 256 experts: 512
-    // assignments 4.1 and 5.7, 2048 5.2 and 6.3, 3072 6.9 and 6.5, 4096 8.6 and 6.6); a warp for every 128 assignments
+    // assignments 4.1 and 5.7, 2048 5.2 and 6.3, 4096 8.6 and 6.6); a warp for every 128 assignments
     const int ranks = a.pairs <= 2048 ? 1 : wide_cluster_fits(config) ? kPlanCluster : 8;
     const int64_t warps = ((int64_t)a.pairs / ranks + 127) / 128;
     const int threads = 128 * (int)std::min<int64_t>(std::max<int64_t>((warps + 3) / 4, 1), 8);
