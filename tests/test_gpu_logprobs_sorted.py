@@ -74,3 +74,23 @@ def test_large_scores_that_lie_together(cuda, rows, vocab, threads, dtype):
             e = vocab / (2 * threads) + 200
             limit = _heads.EPS32 * (e + 7 * (w.abs() + np.log(vocab) + 8))
             assert ((top_lp.double() - w).abs() <= limit).all()
+
+
+def test_more_large_scores_with_one_thread_than_bounds_can_tame(cuda):
+    """15,600 rising scores at the places that the first thread of the first of eight CTAs reads: each bound
+    from what is held passes some 500 of them, so the alternatives are found one by one."""
+    torch = cuda
+    vocab, top = 32_000_001, 20
+    x = torch.empty((1, vocab), device="cuda").normal_(-9.0, 1.0, generator=torch.Generator(device="cuda").manual_seed(1))
+    granule = torch.arange(0, vocab // 8 // 4, 256, device="cuda")
+    at = (granule[:, None] * 4 + torch.arange(4, device="cuda")).flatten()
+    x[0, at] = torch.linspace(1, 9, len(at), device="cuda")
+    assert len(at) > 15_000
+    _, entropy, top_lp, ids = token_logprobs_device(x, top=top)
+    assert torch.equal(ids[0], at.flip(0)[:top])
+    lp = torch.log_softmax(x.double(), dim=1)
+    want = lp[0, ids[0]]
+    e = vocab / (2 * 2048) + 200
+    assert ((top_lp[0].double() - want).abs() <= _heads.EPS32 * (e + 7 * (want.abs() + np.log(vocab) + 8))).all()
+    # y is within 8 + (ln V + 18) / ln 2 of the reference where it has weight; E (1 + 2 M) u as for merged marks
+    assert abs(float(entropy[0]) + float((lp.exp() * lp).sum())) <= _heads.EPS32 * e * (1 + 2 * 60)
